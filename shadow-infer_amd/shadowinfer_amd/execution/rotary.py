@@ -1,0 +1,187 @@
+"""Rotary positions for decoding: pairs in either layout, part of the head, and
+the scalings that stretch a model past the context it was trained on.
+
+``rope_split`` (row_ops.py) is the denoising step's fixed form (half layout,
+whole head, tables in the row dtype, the reference's roundings). Here the angles
+come from the positions themselves in 64 bits, so there is no table and no last
+position, the products are fp32 and every value is rounded once.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+from typing import List, Optional, Tuple, Union
+
+import torch
+
+from .. import _native
+
+_ROWS = ctypes.c_int64 * 9  # si_rotary_rows
+_KINDS = ("linear", "ntk", "yarn", "bands")
+
+
+@dataclass(frozen=True)
+class RotaryScaling:
+    """How the angles per position change for contexts ``factor`` times as long
+    as the ``original_positions`` a model was trained on.
+
+    * ``"linear"``: every angle divided by ``factor`` (position interpolation).
+    * ``"ntk"``: the base times ``factor ** (r / (r - 2))``, r the rotary size, so
+      that the slowest pair is divided by ``factor`` and the fastest kept.
+    * ``"yarn"``: pairs that turn more than ``fast`` times over the original
+      context kept, those that turn less than ``slow`` times divided by
+      ``factor``, a linear ramp over the pair index between; values times
+      ``0.1 ln(factor) + 1`` (Peng et al., arXiv 2309.00071).
+    * ``"bands"``: kept above ``high`` turns over the original context, divided
+      by ``factor`` below ``low``, a ramp that is linear in the turns between.
+    """
+
+    kind: str
+    factor: float
+    original_positions: int = 4096
+    fast: float = 32.0
+    slow: float = 1.0
+    low: float = 1.0
+    high: float = 4.0
+
+    def __post_init__(self) -> None:
+        if self.kind not in _KINDS:
+            raise ValueError(f"scaling kind must be one of {_KINDS}, got {self.kind!r}")
+        if not (math.isfinite(self.factor) and self.factor >= 1.0):
+            raise ValueError(f"factor must be >= 1, got {self.factor}")
+        if self.original_positions < 1:
+            raise ValueError(f"original_positions must be >= 1, got {self.original_positions}")
+        if not (self.fast > self.slow > 0.0 and self.high > self.low > 0.0):
+            raise ValueError("need fast > slow > 0 and high > low > 0")
+
+    def angles(self, size: int, base: float) -> Tuple[List[float], float]:
+        """(radians per position of each of the size / 2 pairs, factor on the
+        values) in Python floats."""
+        if self.kind == "ntk":
+            if size < 4:
+                raise ValueError("ntk scaling needs a rotary size of 4 at least")
+            return _plain(size, base * self.factor ** (size / (size - 2))), 1.0
+        f = _plain(size, base)
+        if self.kind == "linear":
+            return [x / self.factor for x in f], 1.0
+        known = float(self.original_positions)
+        if self.kind == "bands":
+            out = []
+            for x in f:
+                turns = known * x / (2.0 * math.pi)
+                keep = min(1.0, max(0.0, (turns - self.low) / (self.high - self.low)))
+                out.append(keep * x + (1.0 - keep) * (x / self.factor))
+            return out, 1.0
+
+        def pair(turns: float) -> float:  # the pair that turns so often over the known context
+            return size * math.log(known / (2.0 * math.pi * turns)) / (2.0 * math.log(base))
+
+        first = max(math.floor(pair(self.fast)), 0)
+        last = min(math.ceil(pair(self.slow)), size - 1)
+        width = last - first if last != first else 0.001
+        out = []
+        for i, x in enumerate(f):
+            slow = min(1.0, max(0.0, (i - first) / width))
+            out.append(slow * (x / self.factor) + (1.0 - slow) * x)
+        return out, 0.1 * math.log(self.factor) + 1.0
+
+
+def _plain(size: int, base: float) -> List[float]:
+    return [base ** (-2.0 * i / size) for i in range(size // 2)]
+
+
+class RotaryEmbedding:
+    """Rotates the first ``rotary_dim`` values (default: all) of query and key
+    heads by their positions. ``layout``: ``"half"`` pairs value i with
+    i + rotary_dim / 2, ``"interleaved"`` pairs 2i with 2i + 1."""
+
+    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0,
+                 layout: str = "half", scaling: Optional[RotaryScaling] = None,
+                 device: Union[str, torch.device] = "cuda") -> None:
+        size = head_dim if rotary_dim is None else rotary_dim
+        if not 0 < head_dim <= 1024:
+            raise ValueError(f"head_dim must be in 1..1024, got {head_dim}")
+        if size < 2 or size % 2 or size > head_dim:
+            raise ValueError(f"rotary_dim must be even and in 2..{head_dim}, got {size}")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+        if not (math.isfinite(base) and base > 1.0):
+            raise ValueError(f"base must be > 1, got {base}")
+        self.head_dim, self.rotary_dim = int(head_dim), int(size)
+        self.base, self.layout, self.scaling = float(base), layout, scaling
+        angles, self.value_factor = ((_plain(size, base), 1.0) if scaling is None
+                                     else scaling.angles(size, base))
+        self.angles = tuple(angles)  # radians per position of each pair
+        self.device = torch.device(device)
+        # turns per position, in fp64 on the device
+        self.turns = torch.tensor([x / (2.0 * math.pi) for x in angles], dtype=torch.float64,
+                                  device=self.device)
+
+    def _rows(self, x: torch.Tensor, what: str, inplace: bool):
+        if x.dim() not in (3, 4) or x.shape[-1] != self.head_dim:
+            raise ValueError(f"{what} must be [tokens, heads, {self.head_dim}] or "
+                             f"[batch, tokens, heads, {self.head_dim}], got {tuple(x.shape)}")
+        if inplace:
+            if x.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
+                raise ValueError(f"{what} cannot be rotated in place: strides {x.stride()}")
+            out = x
+        else:
+            if x.stride(-1) != 1:
+                x = x.contiguous()
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        s, o = x.stride(), out.stride()
+        sb, ob = (s[0], o[0]) if x.dim() == 4 else (0, 0)
+        return x, out, _ROWS(x.data_ptr(), out.data_ptr(), x.shape[-2], sb, s[-3], s[-2], ob, o[-3],
+                             o[-2])
+
+    def check_positions(self, positions: torch.Tensor, lead: torch.Size,
+                        device: torch.device) -> Tuple[int, int]:
+        """Refuses positions that are not one integer per token of ``lead``
+        (``[S]`` also serves every row of ``[B, S]``); returns their element
+        strides between batches and tokens."""
+        if positions.dtype not in (torch.int64, torch.int32):
+            raise TypeError(f"positions must be int64 or int32, got {positions.dtype}")
+        if positions.device != device:
+            raise ValueError(f"positions must be on {device}, got {positions.device}")
+        if positions.shape != lead and not (len(lead) == 2 and positions.shape == lead[1:]):
+            raise ValueError(f"positions must be {list(lead)}, got {list(positions.shape)}")
+        s = positions.stride()
+        return (s[0] if len(s) == 2 else 0), s[-1]
+
+    def __call__(self, positions: torch.Tensor, q: torch.Tensor, k: Optional[torch.Tensor] = None,
+                 *, transpose: bool = False, inplace: bool = False
+                 ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+        """Rotated ``q``, or ``(q, k)``: tensors ``[T, heads, D]`` or ``[B, S,
+        heads, D]`` (any strides; fp32, fp16 or bf16; the head counts may differ),
+        in one launch. ``positions``: int64 or int32 ``[T]``, ``[B, S]`` or, for
+        every row of a batch, ``[S]``; any value. ``transpose=True`` turns the
+        other way: the gradient of this call with respect to its input, and,
+        where ``value_factor`` is 1, its inverse. ``inplace=True`` writes into q
+        and k. Not recorded by autograd."""
+        _native.require_device(q, "RotaryEmbedding")
+        if self.turns.device != q.device:
+            raise ValueError(f"this RotaryEmbedding is on {self.turns.device}, q on {q.device}")
+        code = _native.dtype_code(q.dtype)
+        lead = q.shape[:-2]
+        if k is not None:
+            if k.dtype != q.dtype or k.device != q.device:
+                raise ValueError("q and k must share device and dtype")
+            if k.shape[:-2] != lead:
+                raise ValueError(f"q and k must hold the same tokens, got {tuple(q.shape)} and "
+                                 f"{tuple(k.shape)}")
+        # sources stay bound until the launch is queued
+        src_q, out_q, rows_q = self._rows(q, "q", inplace)
+        src_k, out_k, rows_k = (None, None, None) if k is None else self._rows(k, "k", inplace)
+        pb, ps = self.check_positions(positions, lead, q.device)
+        B, S = (lead[0], lead[1]) if len(lead) == 2 else (1, lead[0])
+        _native.call_on(q.device, "si_rotary", rows_q, rows_k, code, B, S, self.head_dim,
+                        self.rotary_dim // 2, 1 if self.layout == "interleaved" else 0,
+                        self.turns.data_ptr(), self.value_factor, 1 if transpose else 0,
+                        positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0, pb, ps)
+        return out_q if k is None else (out_q, out_k)
+
+    def __repr__(self) -> str:
+        return (f"RotaryEmbedding(head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, "
+                f"base={self.base}, layout={self.layout!r}, scaling={self.scaling})")

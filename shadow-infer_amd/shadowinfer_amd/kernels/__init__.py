@@ -42,6 +42,9 @@ _KERNELS = (
     "admit_codes_kernel",
     "paged_kv_kernel",
     "step_row_kernel",
+    "rotary_kernel",
+    "page_pool_kernel",
+    "paged_attention_kernel",
 )
 
 # keys of the reference's status dict (kernels/__init__.py:63-70) and whether

@@ -1,10 +1,12 @@
 """Packed mixed-precision KV cache (PackedKVCache), its precision plan, the
-rate-distortion admission that chooses the precisions, and the fused
-packed-KV attention."""
+rate-distortion admission that chooses the precisions, the fused packed-KV
+attention, and the page pool of many sequences with its decode attention."""
 
 from .compress import compress_kv_with_plan
 from .packed_attention import packed_attention
 from .packed_kv_cache import PackedKVCache
+from .page_pool import KVPagePool
+from .paged_attention import paged_attention
 from .paged_kv_store import PagedKVStore
 from .rd_allocator import (
     admit_budget,
@@ -26,6 +28,7 @@ from .precision_plan import (
 __all__ = [
     "CODE_PRECISIONS",
     "EVICTED",
+    "KVPagePool",
     "PRECISION_CODES",
     "PRECISION_ORDER",
     "PackedKVCache",
@@ -39,5 +42,6 @@ __all__ = [
     "kv_sensitivity",
     "map_to_codes",
     "packed_attention",
+    "paged_attention",
     "predict_codes_bytes",
 ]
