@@ -101,8 +101,9 @@ def visible(page_table: torch.Tensor, lengths: torch.Tensor, pages: int, page_si
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
            lengths: torch.Tensor, sm_scale: float, window: Optional[int] = None):
     """``q [B, Hq, D]``, all rows ``k``, ``v [pages, Hk, page_size, D]`` -> fp64
-    (out, lse, weight, reach): ``weight`` = sum p |v| and ``reach`` = the largest
-    sm_scale * sum |q k| of a row's positions, for error bounds."""
+    (out, lse, weight, reach, peak): for error bounds, ``weight`` = sum p |v|, ``reach``
+    = the largest sm_scale * sum |q k| of a row's positions, and ``peak`` = the larger of
+    128 max_t (p_t max_d |v_td|) and max_t p_t max |v|."""
     B, Hq, D = q.shape
     pages, Hk, P, _ = k.shape
     group = Hq // Hk
@@ -110,6 +111,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.
     weight = torch.zeros_like(out)
     lse = torch.full((B, Hq), -math.inf, dtype=torch.float64, device=q.device)
     reach = torch.zeros(B, Hq, dtype=torch.float64, device=q.device)
+    peak = torch.zeros_like(reach)
     for b, places in enumerate(visible(page_table.cpu(), lengths.cpu(), pages, P, window)):
         if not places:
             continue
@@ -123,4 +125,6 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.
             out[b, h] = p @ vh
             weight[b, h] = p @ vh.abs()
             reach[b, h] = abs(sm_scale) * (kh.abs() @ x.abs()).max()
-    return out, lse, weight, reach
+            row = vh.abs().amax(1)
+            peak[b, h] = torch.maximum(128 * (p * row).max(), p.max() * row.max())
+    return out, lse, weight, reach, peak

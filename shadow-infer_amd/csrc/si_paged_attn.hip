@@ -107,6 +107,13 @@ __device__ __forceinline__ int span_tiles(const AttnArgs& a, int b, int32_t* lo,
   return si_span_tiles(*lo, *hi, kTile);
 }
 
+// A value that is the same in every lane, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // Sum over the block of v, and over the threads before this one.
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int64_t* before) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -124,117 +131,632 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int64_t* 
   }
   __syncthreads();
   *before = base + s - v;
-  return total;
+  return uniform(total);
 }
 
-// A wave's running softmax over its positions: lane (r, kq) = (lane % 16, lane / 16)
-// has query row r's maximum and sum over the positions of its kq, and the
-// output's values d = (4 kq + i) J + j in o[j][i].
+// A wave's running softmax over its positions: lane (c, kq) = (lane % 16, lane / 16)
+// has query row c's maximum (the same in all four kq) and sum over the positions of
+// its kq, and the output's values d = (4 kq + i) J + j in o[j][i], all relative to
+// 2^m.
 template <int J>
 struct Running {
   float m, l;
   f32x4 o[J];
 };
 
-// Products in fp32 (v_mfma_f32_16x16x4_f32): A holds one k of 16 rows, so the
-// scores are K times q transposed, [position][query row], and a lane has the
-// scores of its own row at positions s * 16 + 4 kq + i. The probabilities are then
-// in place as the second product's operand when its k runs over kq, and the
-// output is V transposed times P, [d][query row]. Nothing passes between lanes
-// but the row maxima.
-template <int KIND, int DP>
-__device__ __forceinline__ void wave_tile(const AttnArgs& a, const float* q, int b, int hk, int32_t t0,
-                                          int32_t hi, Running<DP / 16>& st) {
-  constexpr int J = DP / 16, M = DP / 32;
-  const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
-  // row of position t0 + lane % 32, and its scales (K's in the lower lanes, V's above)
-  const int32_t t = t0 + (lane & 31);
-  int32_t row = -1;
-  if (t < hi) {
-    const uint32_t pg = (uint32_t)t / (uint32_t)a.P;
-    row = si_page_row(a.table[b * a.ts + pg], a.pages, hk, a.Hk, t - (int32_t)pg * a.P, a.P);
-  }
-  float sc = 0.0f;
-  if (KIND == kI8 && row >= 0) sc = load_any(a.pool[lane < 32 ? 2 : 3], a.sdt, row);
-  const int G = KIND == kI4 ? a.D / a.g : 1;
-  f32x4 acc[2] = {};
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int32_t kr = __shfl(row, s * 16 + c, 64);
-    const int64_t base = (int64_t)(kr < 0 ? 0 : kr);
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The larger of a lane's value and those of the lanes 16, 32 and 48 away.
+__device__ __forceinline__ float max_over_kq(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  const float w = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(w), __float_as_uint(w), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// ---------------------------------------------------------------------------
+// Products in fp32 (v_mfma_f32_16x16x4_f32), for fp32 queries or fp32 rows: A holds
+// one k of 16 rows, so the scores are K times q transposed, [position][query row],
+// and a lane has the scores of its own row at positions s * 16 + 4 kq + i. The
+// weights are then in place as the second product's operand when its k runs over
+// kq, and the output is V transposed times P, [d][query row]. Nothing passes
+// between lanes but the row maxima.
+// ---------------------------------------------------------------------------
+template <int KIND, int DP_>
+struct Engine32 {
+  static constexpr int DP = DP_, J = DP / 16, M = DP / 32, kLds = 0;
+  Running<J> st;
+  float q[M * 8];
+
+  __device__ __forceinline__ void begin(const AttnArgs& a, int b, int64_t head0, int rows) {
+    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const int d = (m * 4 + kq) * 8;
-      float x[8] = {};
-      if (d < a.D) {
-        load_row<KIND, 8>(a.pool[0], base * a.D + d, x);
-        if constexpr (KIND == kI4) {
-          const float ks = load_any(a.pool[2], a.sdt, base * G + d / a.g);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= ks;
-        }
+      for (int e = 0; e < 8; ++e) {
+        const int d = (m * 4 + kq) * 8 + e;
+        q[m * 8 + e] = c < rows && d < a.D
+                           ? load_any(a.q, a.qdt, b * a.qs[0] + (head0 + c) * a.qs[1] + d) : 0.0f;
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        acc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], q[m * 8 + e], acc[s], 0, 0, 0);
     }
   }
-  int32_t vr[2][4];
-  float p[2][4], top = st.m;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      vr[s][i] = __shfl(row, s * 16 + kq * 4 + i, 64);
-      float x = acc[s][i] * a.scale;
-      if constexpr (KIND == kI8) x *= __shfl(sc, s * 16 + kq * 4 + i, 64);
-      p[s][i] = vr[s][i] < 0 ? -INFINITY : x;
-      top = fmaxf(top, p[s][i]);
+
+  // The wave's positions of tiles [ta, tb).
+  __device__ __forceinline__ void walk(const AttnArgs& a, char*, int b, int hk, int32_t lo, int32_t hi,
+                                       int32_t ta, int32_t tb) {
+    for (int32_t i = ta; i < tb; ++i) {
+      const int32_t t0 = lo + i * kTile + (threadIdx.x >> 6) * kWaveTokens;
+      if (t0 < hi) tile(a, b, hk, t0, hi);
     }
   }
-  top = fmaxf(top, __shfl_xor(top, 16, 64));
-  top = fmaxf(top, __shfl_xor(top, 32, 64));
-  const float ref = top == -INFINITY ? 0.0f : top;  // nothing yet: every weight below is 0
-  const float keep = __builtin_amdgcn_exp2f(st.m - ref);
-  st.m = top;
-  st.l *= keep;
-#pragma unroll
-  for (int j = 0; j < J; ++j) st.o[j] *= keep;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool live = vr[s][i] >= 0;
-      float w = __builtin_amdgcn_exp2f(p[s][i] - ref);
-      st.l += w;
-      if constexpr (KIND == kI8) {
-        const float vs = __shfl(sc, 32 + s * 16 + kq * 4 + i, 64);
-        w *= vs;
-      }
-      const int64_t base = live ? vr[s][i] : 0;
-      const int d = c * J;
-      float x[J] = {};
-      if (live && d < a.D) {  // rows that take no part count as zeros, whatever they hold
-        load_row<KIND, J>(a.pool[1], base * a.D + d, x);
-        if constexpr (KIND == kI4) {
-          const float vs = load_any(a.pool[3], a.sdt, base * G + d / a.g);
-#pragma unroll
-          for (int j = 0; j < J; ++j) x[j] *= vs;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-        st.o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], w, st.o[j], 0, 0, 0);
+
+  __device__ __forceinline__ void tile(const AttnArgs& a, int b, int hk, int32_t t0, int32_t hi) {
+    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
+    // row of position t0 + lane % 32, and its scales (K's in the lower lanes, V's above)
+    const int32_t t = t0 + (lane & 31);
+    int32_t row = -1;
+    if (t < hi) {
+      const uint32_t pg = (uint32_t)t / (uint32_t)a.P;
+      row = si_page_row(a.table[b * a.ts + pg], a.pages, hk, a.Hk, t - (int32_t)pg * a.P, a.P);
     }
+    float sc = 0.0f;
+    if (KIND == kI8 && row >= 0) sc = load_any(a.pool[lane < 32 ? 2 : 3], a.sdt, row);
+    const int G = KIND == kI4 ? a.D / a.g : 1;
+    f32x4 acc[2] = {};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int32_t kr = __shfl(row, s * 16 + c, 64);
+      const int64_t base = (int64_t)(kr < 0 ? 0 : kr);
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const int d = (m * 4 + kq) * 8;
+        float x[8] = {};
+        if (d < a.D) {
+          load_row<KIND, 8>(a.pool[0], base * a.D + d, x);
+          if constexpr (KIND == kI4) {
+            const float ks = load_any(a.pool[2], a.sdt, base * G + d / a.g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= ks;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          acc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], q[m * 8 + e], acc[s], 0, 0, 0);
+      }
+    }
+    int32_t vr[2][4];
+    float p[2][4], top = st.m;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        vr[s][i] = __shfl(row, s * 16 + kq * 4 + i, 64);
+        float x = acc[s][i] * a.scale;
+        if constexpr (KIND == kI8) x *= __shfl(sc, s * 16 + kq * 4 + i, 64);
+        p[s][i] = vr[s][i] < 0 ? -INFINITY : x;
+        top = fmaxf(top, p[s][i]);
+      }
+    }
+    top = max_over_kq(top);
+    const float ref = top == -INFINITY ? 0.0f : top;  // nothing yet: every weight below is 0
+    const float keep = __builtin_amdgcn_exp2f(st.m - ref);
+    st.m = top;
+    st.l *= keep;
+#pragma unroll
+    for (int j = 0; j < J; ++j) st.o[j] *= keep;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool live = vr[s][i] >= 0;
+        float w = __builtin_amdgcn_exp2f(p[s][i] - ref);
+        st.l += w;
+        if constexpr (KIND == kI8) {
+          const float vs = __shfl(sc, 32 + s * 16 + kq * 4 + i, 64);
+          w *= vs;
+        }
+        const int64_t base = live ? vr[s][i] : 0;
+        const int d = c * J;
+        float x[J] = {};
+        if (live && d < a.D) {  // rows that take no part count as zeros, whatever they hold
+          load_row<KIND, J>(a.pool[1], base * a.D + d, x);
+          if constexpr (KIND == kI4) {
+            const float vs = load_any(a.pool[3], a.sdt, base * G + d / a.g);
+#pragma unroll
+            for (int j = 0; j < J; ++j) x[j] *= vs;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          st.o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], w, st.o[j], 0, 0, 0);
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Products on 16-bit operands (v_mfma_f32_16x16x32), for 16-bit queries over
+// 16-bit, int8 and int4 rows, the layout of Engine32 with eight k per lane. What
+// keeps this as exact as fp32 weights would be:
+//  * int8 and int4 codes are exact in fp16 (0x6400 | u is 1024 + u); a row's int8
+//    scale multiplies its score, and its value's scale the weight, in fp32;
+//  * an int4 group's scale is split as 2^e (e from the row's largest group, in fp32
+//    like an int8 scale) times s' < 2. n s' has 3 + 8 bits for a bf16 scale, so it is
+//    exact in fp16; fp16 and fp32 scales are carried as two such parts (NS = 2);
+//  * query rows are scaled by a power of two so that their largest value is in
+//    [2^14, 2^15): bf16's 8 bits are then exact in fp16 over 2^32. fp16 queries over
+//    bf16 rows are two bf16 parts (NQ = 2), again exact;
+//  * weights w = exp(s - m) sv are two 16-bit parts, hi and what hi leaves. Their
+//    reference m is the maximum of s + log2(sv), so w is at most 2^14 whatever the
+//    rows' scales are, and the parts hold it to 2^-22 (fp16) or 2^-16 (bf16).
+// The k order within a chunk of eight is free as long as both operands have the
+// same: int4's nibbles come out as 1 5 0 4 3 7 2 6.
+//
+// HBM bounds it: each wave has the next tile's rows in flight while it works on
+// one (two register buffers), rows and scales of a tile go through LDS.
+// ---------------------------------------------------------------------------
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ h2 as_h2(uint32_t u) { return __builtin_bit_cast(h2, u); }
+__device__ __forceinline__ uint32_t as_u32(h2 h) { return __builtin_bit_cast(uint32_t, h); }
+__device__ __forceinline__ h2 pair(float x) { return h2{(_Float16)x, (_Float16)x}; }
+
+template <int WORDS>
+__device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
+  if constexpr (WORDS == 0) {
+    w[0] = *reinterpret_cast<const uint16_t*>(p);  // four int4 codes
+  } else if constexpr (WORDS % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4) {
+      const u4 x = *reinterpret_cast<const u4*>(p + 4 * i);
+      w[i] = x[0]; w[i + 1] = x[1]; w[i + 2] = x[2]; w[i + 3] = x[3];
+    }
+  } else if constexpr (WORDS == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x; w[1] = x.y;
+  } else {
+    static_assert(WORDS == 1, "half a word, a word, two, or whole 16 bytes");
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
+// EXACT: D == DP, and wider loads of K.
+template <int KIND, int DP_, bool EXACT, int NQ, int NS>
+struct Engine16 {
+  static constexpr int DP = DP_, J = DP / 16, M = DP / 32;
+  static constexpr bool kBf = KIND == kBF16;
+  static constexpr bool kScaled = KIND == kI8 || KIND == kI4;
+  static constexpr int kG = 8;  // int4 groups of a row at most
+  // bits of a value; words of K per lane and 16 positions, of V per lane and position
+  static constexpr int kBits = KIND == kI4 ? 4 : KIND == kI8 ? 8 : 16;
+  static constexpr int kKW = DP / 4 * kBits / 32, kVW = J * kBits / 32;  // 0: half a word
+  static constexpr int kVW1 = kVW ? kVW : 1;
+  static constexpr int kUnit = 8 * kBits / 32;  // words of eight values
+
+  // A wave's LDS: rows [2][32], then per position: K's factor, V's factor, its
+  // logarithm, and int4's s' as [32][kG] for K and [kG][32] for V, NS parts each.
+  static constexpr int kLdsScale = 2 * 32 * 4;
+  static constexpr int kLdsParts = kLdsScale + (kScaled ? 3 * 32 * 4 : 0);
+  static constexpr int kLds = kLdsParts + (KIND == kI4 ? 2 * NS * 32 * kG * 2 : 0);
+
+  struct Tile {
+    uint32_t k[2][kKW], v[2][4][kVW1];
+    uint32_t sc[KIND == kI4 ? (NS == 1 ? 4 : 8) : 1];
+    int32_t row;    // of position lane % 32
+    uint32_t live;  // bit 4 s + i: position s * 16 + 4 kq + i takes part
+  };
+
+  Running<J> st;
+  u4 q[NQ][M];
+  float qscale;  // what scores are multiplied by: scale * log2(e) / the row's power of two
+
+  // Value e (in operand order) of chunk m: its d.
+  __device__ __forceinline__ static int chunk_d(int m, int kq) {
+    if constexpr (EXACT && KIND == kI8) return (m >> 1) * 64 + kq * 16 + (m & 1) * 8;
+    if constexpr (EXACT && KIND == kI4) return kq * (DP / 4) + m * 8;
+    return (m * 4 + kq) * 8;
+  }
+
+  __device__ __forceinline__ void begin(const AttnArgs& a, int b, int64_t head0, int rows) {
+    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
+    float x[M][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        constexpr int order[8] = {1, 5, 0, 4, 3, 7, 2, 6};
+        const int d = chunk_d(m, kq) + (KIND == kI4 ? order[e] : e);
+        x[m][e] = c < rows && d < a.D
+                      ? load_any(a.q, a.qdt, b * a.qs[0] + (head0 + c) * a.qs[1] + d) : 0.0f;
+        top = fmaxf(top, fabsf(x[m][e]));
+      }
+    }
+    qscale = a.scale;
+    if constexpr (!kBf) {
+      top = max_over_kq(top);
+      int up = 0;  // a power of two for the row
+      if (top > 0.0f && top < INFINITY) up = 15 - __builtin_amdgcn_frexp_expf(top);
+      qscale = __builtin_amdgcn_ldexpf(a.scale, -up);
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+          q[0][m][e / 2] = as_u32(h2{(_Float16)__builtin_amdgcn_ldexpf(x[m][e], up),
+                                     (_Float16)__builtin_amdgcn_ldexpf(x[m][e + 1], up)});
+      }
+    } else {
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const uint32_t hi = f32x2_to_bf16x2_bits(x[m][e], x[m][e + 1]);
+          q[0][m][e / 2] = hi;
+          if constexpr (NQ == 2)
+            q[1][m][e / 2] = f32x2_to_bf16x2_bits(x[m][e] - __uint_as_float(hi << 16),
+                                                  x[m][e + 1] - __uint_as_float(hi & 0xffff0000u));
+        }
+      }
+    }
+  }
+
+  // The page table entry of position t0 + lane % 32.
+  __device__ __forceinline__ static int32_t entry(const AttnArgs& a, int b, int32_t t0, int32_t hi) {
+    const int32_t t = t0 + (threadIdx.x & 31);
+    return t < hi ? a.table[b * a.ts + (uint32_t)t / (uint32_t)a.P] : -1;
+  }
+
+  // Starts the loads of a tile. Positions that do not take part read row 0.
+  __device__ __forceinline__ static void start(const AttnArgs& a, int32_t* lds_rows, int hk, int32_t t0,
+                                               int32_t hi, int32_t page, Tile& x) {
+    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
+    const int32_t t = t0 + (lane & 31);
+    x.row = t < hi ? si_page_row(page, a.pages, hk, a.Hk, (int32_t)((uint32_t)t % (uint32_t)a.P), a.P) : -1;
+    if (lane < 32) lds_rows[lane] = x.row;
+    wave_sync();
+    const char* kp = reinterpret_cast<const char*>(a.pool[0]);
+    const char* vp = reinterpret_cast<const char*>(a.pool[1]);
+    const int64_t row_bytes = (int64_t)a.D * kBits / 8;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int32_t r = lds_rows[s * 16 + c];
+      const char* p = kp + (r < 0 ? 0 : r) * row_bytes;
+      if constexpr (EXACT) {
+        // 16 bytes a load: 64 bytes of a row by its four lanes
+        if constexpr (kBits == 16) {
+#pragma unroll
+          for (int m = 0; m < M; ++m) load_words<4>(p + chunk_d(m, kq) * 2, x.k[s] + 4 * m);
+        } else if constexpr (kBits == 8) {
+#pragma unroll
+          for (int m = 0; m < M; m += 2) load_words<4>(p + chunk_d(m, kq), x.k[s] + 2 * m);
+        } else {
+          load_words<kKW>(p + chunk_d(0, kq) / 2, x.k[s]);
+        }
+      } else {
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const int d = chunk_d(m, kq);
+          if (d < a.D) {
+            load_words<kUnit>(p + d * kBits / 8, x.k[s] + kUnit * m);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kUnit; ++i) x.k[s][kUnit * m + i] = KIND == kI4 ? 0x88888888u : 0u;
+          }
+        }
+      }
+    }
+    x.live = 0;
+    const bool in = EXACT || c * J < a.D;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int4 r4 = *reinterpret_cast<const int4*>(lds_rows + s * 16 + kq * 4);
+      const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r[i] >= 0) x.live |= 1u << (4 * s + i);
+        const char* p = vp + (r[i] < 0 ? 0 : r[i]) * row_bytes + c * J * kBits / 8;
+        if (in) {
+          load_words<kVW>(p, x.v[s][i]);
+        } else {
+#pragma unroll
+          for (int w = 0; w < kVW1; ++w) x.v[s][i][w] = KIND == kI4 ? 0x88888888u : 0u;
+        }
+      }
+    }
+    if constexpr (kScaled) {  // K's scales in the lower lanes, V's in the upper
+      const int64_t r = x.row < 0 ? 0 : x.row;
+      const void* sp = a.pool[lane < 32 ? 2 : 3];
+      if constexpr (KIND == kI8) {
+        x.sc[0] = a.sdt == SI_DT_F32 ? reinterpret_cast<const uint32_t*>(sp)[r]
+                                     : reinterpret_cast<const uint16_t*>(sp)[r];
+      } else {
+        const int G = a.D / a.g;
+        if constexpr (NS == 1) {  // bf16
+          if (G == 8) {
+            load_words<4>(reinterpret_cast<const char*>(sp) + r * 16, x.sc);
+          } else {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint16_t* h = reinterpret_cast<const uint16_t*>(sp) + r * G + 2 * w;
+              const uint32_t lo = 2 * w < G ? h[0] : 0, hi16 = 2 * w + 1 < G ? h[1] : 0;
+              x.sc[w] = lo | (hi16 << 16);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < 8; ++w) {
+            if (w >= G) x.sc[w] = 0;
+            else if (a.sdt == SI_DT_F32) x.sc[w] = reinterpret_cast<const uint32_t*>(sp)[r * G + w];
+            else x.sc[w] = __float_as_uint(load_any(sp, a.sdt, r * G + w));
+          }
+        }
+      }
+    }
+  }
+
+  // A tile's scales into the wave's LDS.
+  __device__ __forceinline__ static void place_scales(const AttnArgs& a, char* lds, const Tile& x) {
+    const int lane = threadIdx.x & 63, t = lane & 31;
+    float* factor = reinterpret_cast<float*>(lds + kLdsScale);  // [3][32]
+    float f;
+    if constexpr (KIND == kI8) {
+      f = a.sdt == SI_DT_F32 ? __uint_as_float(x.sc[0])
+          : a.sdt == SI_DT_BF16 ? bf16_bits_to_f32(x.sc[0]) : f16_bits_to_f32(x.sc[0]);
+      if (x.row < 0) f = 0.0f;
+    } else {
+      float s[kG], top = 0.0f;
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        if constexpr (NS == 1) s[g] = __uint_as_float(g & 1 ? x.sc[g / 2] & 0xffff0000u : x.sc[g / 2] << 16);
+        else s[g] = __uint_as_float(x.sc[g]);
+        if (x.row < 0) s[g] = 0.0f;
+        top = fmaxf(top, s[g]);
+      }
+      // s' = s / 2^e < 2; a row of infinities keeps e within fp32
+      const int e = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+      f = __builtin_amdgcn_ldexpf(1.0f, e);
+      _Float16* part = reinterpret_cast<_Float16*>(lds + kLdsParts) + (lane < 32 ? 0 : NS * 32 * kG);
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        const float r = __builtin_amdgcn_ldexpf(s[g], -e);
+        const int at = lane < 32 ? t * kG + g : g * 32 + t;
+        if constexpr (NS == 1) {
+          part[at] = (_Float16)r;
+        } else {
+          const float hi = bf16_bits_to_f32(f32_to_bf16_bits(r));
+          part[at] = (_Float16)hi;
+          part[32 * kG + at] = (_Float16)(hi < INFINITY ? r - hi : 0.0f);
+        }
+      }
+    }
+    if (lane < 32) {
+      factor[t] = f;
+    } else {
+      factor[32 + t] = f;
+      // (a scale below 2^-80 or not a number: its weight needs no more room than this)
+      factor[64 + t] = fminf(fmaxf(__builtin_amdgcn_logf(f), -80.0f), 127.0f);
+    }
+    wave_sync();
+  }
+
+  // Chunk m of K, positions s * 16 + c, as the first product's operand; part p.
+  __device__ __forceinline__ static u4 k_operand(const Tile& x, int s, int m, h2 scale) {
+    if constexpr (kBits == 16) return u4{x.k[s][4 * m], x.k[s][4 * m + 1], x.k[s][4 * m + 2], x.k[s][4 * m + 3]};
+    u4 r;
+    if constexpr (KIND == kI8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t u = x.k[s][2 * m + i] ^ 0x80808080u;
+        r[2 * i] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - pair(1152.0f));
+        r[2 * i + 1] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - pair(1152.0f));
+      }
+    } else {
+      const uint32_t u = x.k[s][m], w = u >> 8;
+      r[0] = as_u32((as_h2((u & 0x000f000fu) | 0x64006400u) - pair(1032.0f)) * scale);
+      r[1] = as_u32((as_h2((u & 0x00f000f0u) | 0x64006400u) * pair(0.0625f) - pair(72.0f)) * scale);
+      r[2] = as_u32((as_h2((w & 0x000f000fu) | 0x64006400u) - pair(1032.0f)) * scale);
+      r[3] = as_u32((as_h2((w & 0x00f000f0u) | 0x64006400u) * pair(0.0625f) - pair(72.0f)) * scale);
+    }
+    return r;
+  }
+
+  // Values kJG * i .. of two positions, paired: out[j] = (a's value, b's value).
+  static constexpr int kJG = KIND == kI8 ? 4 : 2;
+  __device__ __forceinline__ static void v_pairs(const uint32_t* a, const uint32_t* b, int i, uint32_t* out) {
+    if constexpr (kBits == 16) {
+      out[0] = __builtin_amdgcn_perm(b[i], a[i], 0x05040100u);
+      out[1] = __builtin_amdgcn_perm(b[i], a[i], 0x07060302u);
+    } else if constexpr (KIND == kI8) {
+      const uint32_t lo = __builtin_amdgcn_perm(b[i], a[i], 0x05010400u) ^ 0x80808080u;
+      const uint32_t hi = __builtin_amdgcn_perm(b[i], a[i], 0x07030602u) ^ 0x80808080u;
+      out[0] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u)) - pair(1152.0f));
+      out[1] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u)) - pair(1152.0f));
+      out[2] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u)) - pair(1152.0f));
+      out[3] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u)) - pair(1152.0f));
+    } else {  // byte i: values 2i (high nibble) and 2i + 1
+      const uint32_t u = __builtin_amdgcn_perm(b[0], a[0], 0x0c040c00u + 0x00010001u * i);
+      out[0] = as_u32(as_h2((u & 0x00f000f0u) | 0x64006400u) * pair(0.0625f) - pair(72.0f));
+      out[1] = as_u32(as_h2((u & 0x000f000fu) | 0x64006400u) - pair(1032.0f));
+    }
+  }
+
+  __device__ __forceinline__ static f32x4 mma(u4 x, u4 y, f32x4 z) {
+    if constexpr (kBf)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), z, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), z, 0, 0, 0);
+  }
+
+  __device__ __forceinline__ void work(const AttnArgs& a, char* lds, const Tile& x) {
+    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
+    const float* factor = reinterpret_cast<const float*>(lds + kLdsScale);
+    const _Float16* kpart = reinterpret_cast<const _Float16*>(lds + kLdsParts);
+    const _Float16* vpart = kpart + NS * 32 * kG;
+    if constexpr (kScaled) place_scales(a, lds, x);
+
+    f32x4 acc[2] = {};
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+#pragma unroll
+        for (int p = 0; p < (KIND == kI4 ? NS : 1); ++p) {
+          h2 ks = {};
+          if constexpr (KIND == kI4) {
+            const int d = chunk_d(m, kq);
+            const int g = EXACT || d < a.D ? d / a.g : 0;
+            const _Float16 f = kpart[p * 32 * kG + (s * 16 + c) * kG + g];
+            ks = h2{f, f};
+          }
+          const u4 ko = k_operand(x, s, m, ks);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) acc[s] = mma(ko, q[n][m], acc[s]);
+        }
+      }
+    }
+
+    float w[8], y[8], top = st.m;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      f32x4 kf = {1.0f, 1.0f, 1.0f, 1.0f}, lg = {0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (kScaled) {
+        kf = *reinterpret_cast<const f32x4*>(factor + s * 16 + kq * 4);
+        lg = *reinterpret_cast<const f32x4*>(factor + 64 + s * 16 + kq * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v = acc[s][i] * qscale;
+        if constexpr (kScaled) v *= kf[i];
+        if (!(x.live >> (4 * s + i) & 1)) v = -INFINITY;
+        y[4 * s + i] = v;
+        top = fmaxf(top, v + lg[i]);
+      }
+    }
+    top = max_over_kq(top);
+    if (__any(top > st.m)) {
+      const float keep = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m - top);
+      st.l *= keep;
+#pragma unroll
+      for (int j = 0; j < J; ++j) st.o[j] *= keep;
+      st.m = top;
+    }
+    const float ref = st.m == -INFINITY ? 0.0f : st.m - kRoom;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      f32x4 vf = {1.0f, 1.0f, 1.0f, 1.0f};
+      if constexpr (kScaled) vf = *reinterpret_cast<const f32x4*>(factor + 32 + s * 16 + kq * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = __builtin_amdgcn_exp2f(y[4 * s + i] - ref);
+        st.l += e;
+        w[4 * s + i] = kScaled ? e * vf[i] : e;
+      }
+    }
+    u4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float u = w[2 * i], v = w[2 * i + 1];
+      if constexpr (kBf) {
+        hi[i] = f32x2_to_bf16x2_bits(u, v);
+        lo[i] = f32x2_to_bf16x2_bits(u - __uint_as_float(hi[i] << 16), v - __uint_as_float(hi[i] & 0xffff0000u));
+      } else {
+        const h2 h = {(_Float16)u, (_Float16)v};
+        hi[i] = as_u32(h);
+        lo[i] = as_u32(h2{(_Float16)(u - (float)h.x), (_Float16)(v - (float)h.y)});
+      }
+    }
+
+    uint2 vs[NS][2];
+    if constexpr (KIND == kI4) {
+      const int g = EXACT || c * J < a.D ? c * J / a.g : 0;
+#pragma unroll
+      for (int p = 0; p < NS; ++p)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          vs[p][s] = *reinterpret_cast<const uint2*>(vpart + p * 32 * kG + g * 32 + s * 16 + kq * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < J / kJG; ++i) {
+      uint32_t vv[4][kJG];  // [pair of positions][value]
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        v_pairs(x.v[t >> 1][2 * (t & 1)], x.v[t >> 1][2 * (t & 1) + 1], i, vv[t]);
+        if constexpr (kBits == 16) {
+          // rows that take no part count as zeros, whatever they hold
+          if (x.live != 0xffu) {
+            const uint32_t mask = (x.live >> (2 * t) & 1 ? 0xffffu : 0u) | (x.live >> (2 * t + 1) & 1 ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int j = 0; j < kJG; ++j) vv[t][j] &= mask;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kJG; ++j) {
+        f32x4& o = st.o[i * kJG + j];
+        if constexpr (KIND == kI4) {
+#pragma unroll
+          for (int p = 0; p < NS; ++p) {
+            const u4 vo = {as_u32(as_h2(vv[0][j]) * as_h2(vs[p][0].x)), as_u32(as_h2(vv[1][j]) * as_h2(vs[p][0].y)),
+                           as_u32(as_h2(vv[2][j]) * as_h2(vs[p][1].x)), as_u32(as_h2(vv[3][j]) * as_h2(vs[p][1].y))};
+            o = mma(vo, hi, o);
+            o = mma(vo, lo, o);
+          }
+        } else {
+          const u4 vo = {vv[0][j], vv[1][j], vv[2][j], vv[3][j]};
+          o = mma(vo, hi, o);
+          o = mma(vo, lo, o);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void walk(const AttnArgs& a, char* lds, int b, int hk, int32_t lo, int32_t hi,
+                                       int32_t ta, int32_t tb) {
+    int32_t t0 = lo + ta * kTile + (threadIdx.x >> 6) * kWaveTokens;
+    const int32_t end = tb * (int64_t)kTile + lo < hi ? lo + tb * kTile : hi;
+    if (t0 >= end) return;
+    int32_t* rows = reinterpret_cast<int32_t*>(lds);
+    Tile x, z;
+    start(a, rows, hk, t0, hi, entry(a, b, t0, hi), x);
+    int32_t page = entry(a, b, t0 + kTile, hi);
+    while (true) {
+      t0 += kTile;
+      if (t0 < end) {
+        start(a, rows + 32, hk, t0, hi, page, z);
+        page = entry(a, b, t0 + kTile, hi);
+      }
+      work(a, lds, x);
+      if (t0 >= end) break;
+      t0 += kTile;
+      if (t0 < end) {
+        start(a, rows, hk, t0, hi, page, x);
+        page = entry(a, b, t0 + kTile, hi);
+      }
+      work(a, lds, z);
+      if (t0 >= end) break;
+    }
+    // the sums above are of weights scaled by 2^kRoom
+    st.m -= kRoom;
+  }
+  static constexpr float kRoom = 14.0f;
+};
+
 // DEALT: tiles dealt evenly to kParts blocks, partial results in a.parts. Otherwise
 // block = item, which it finishes.
-template <int KIND, int DP, bool DEALT>
+template <class E, bool DEALT>
 __global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
-  constexpr int J = DP / 16, M = DP / 32;
-  __shared__ float lds_o[4][kRows][DP + 4];
+  constexpr int DP = E::DP, J = DP / 16;
+  // the waves' own memory while they walk, their outputs afterwards
+  constexpr int kOut = kRows * (DP + 4) * (int)sizeof(float);
+  __shared__ __attribute__((aligned(16))) char lds[4 * (kOut > E::kLds ? kOut : E::kLds)];
+  float (*lds_o)[kRows][DP + 4] = reinterpret_cast<float (*)[kRows][DP + 4]>(lds);
   __shared__ float lds_m[4][kRows], lds_l[4][kRows];
   __shared__ int64_t lds_scan[8];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -271,9 +793,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
       }
     }
     __syncthreads();
-    b = (int)lds_scan[4];
-    item = (int)lds_scan[5];
-    ta = (int32_t)lds_scan[6];
+    b = (int)uniform(lds_scan[4]);
+    item = (int)uniform(lds_scan[5]);
+    ta = (int32_t)uniform(lds_scan[6]);
   } else {
     b = blockIdx.x / per;
     item = blockIdx.x - b * per;
@@ -287,30 +809,19 @@ __global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
     const int rows = a.group - rb * kRows < kRows ? a.group - rb * kRows : kRows;
     const int64_t head0 = (int64_t)hk * a.group + rb * kRows;
 
-    Running<J> st;
+    E e;
+    Running<J>& st = e.st;
     st.m = -INFINITY;
     st.l = 0.0f;
 #pragma unroll
     for (int j = 0; j < J; ++j) st.o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float q[M * 8];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = (m * 4 + kq) * 8 + e;
-        q[m * 8 + e] = c < rows && d < a.D
-                           ? load_any(a.q, a.qdt, b * a.qs[0] + (head0 + c) * a.qs[1] + d) : 0.0f;
-      }
-    }
-    for (int32_t i = ta; i < tb; ++i) {
-      const int32_t t0 = lo + i * kTile + wave * kWaveTokens;
-      if (t0 < hi) wave_tile<KIND, DP>(a, q, b, hk, t0, hi, st);
-    }
+    e.begin(a, b, head0, rows);
+    e.walk(a, lds + wave * E::kLds, b, hk, lo, hi, ta, tb);
 
     // the four waves' results together
     st.l += __shfl_xor(st.l, 16, 64);
     st.l += __shfl_xor(st.l, 32, 64);
-    __syncthreads();  // the previous item's results have been read
+    __syncthreads();  // the waves' own memory is free
     if (kq == 0) {
       lds_m[wave][c] = st.m;
       lds_l[wave][c] = st.l;
@@ -352,6 +863,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
     if (!DEALT) return;
     f += tb - ta;
     if (f >= end) return;
+    __syncthreads();  // the results have been read
     ta = 0;
     if (++item == per) {
       item = 0;
@@ -483,22 +995,30 @@ bool dealt(int64_t capacity, int64_t window) {
   return most > kTile;
 }
 
-template <int KIND, int DP>
+template <class E>
 int launch(const AttnArgs& a, bool deal, hipStream_t st) {
   const int64_t items = (int64_t)a.B * a.Hk * a.rb;
   if (deal) {
-    paged_attn<KIND, DP, true><<<kParts, 256, 0, st>>>(a);
+    paged_attn<E, true><<<kParts, 256, 0, st>>>(a);
     const int rows = a.group < kRows ? a.group : kRows;
     paged_join<<<dim3((unsigned)items, (unsigned)rows), a.D <= 64 ? 64 : 128, 0, st>>>(a);
   } else {
-    paged_attn<KIND, DP, false><<<(unsigned)items, 256, 0, st>>>(a);
+    paged_attn<E, false><<<(unsigned)items, 256, 0, st>>>(a);
   }
   return check_launch("si_paged_attn");
 }
 
 template <int KIND>
-int launch_kind(const AttnArgs& a, bool deal, hipStream_t st) {
-  return a.D <= 64 ? launch<KIND, 64>(a, deal, st) : launch<KIND, 128>(a, deal, st);
+int launch32(const AttnArgs& a, bool deal, hipStream_t st) {
+  return a.D <= 64 ? launch<Engine32<KIND, 64>>(a, deal, st) : launch<Engine32<KIND, 128>>(a, deal, st);
+}
+
+template <int KIND, int NQ, int NS>
+int launch16(const AttnArgs& a, bool deal, hipStream_t st) {
+  if (a.D == 64) return launch<Engine16<KIND, 64, true, NQ, NS>>(a, deal, st);
+  if (a.D == 128) return launch<Engine16<KIND, 128, true, NQ, NS>>(a, deal, st);
+  return a.D < 64 ? launch<Engine16<KIND, 64, false, NQ, NS>>(a, deal, st)
+                  : launch<Engine16<KIND, 128, false, NQ, NS>>(a, deal, st);
 }
 
 }  // namespace
@@ -528,7 +1048,7 @@ extern "C" int si_paged_attn(const void* q, int q_dtype, int64_t B, int64_t Hq, 
   SI_CHECK_ARG(pages > 0 && page_size > 0 && pages < ((int64_t)1 << 31) && page_size < ((int64_t)1 << 31) &&
                pages <= (((int64_t)1 << 31) - 1) / Hk / page_size,
                "si_paged_attn: pools hold fewer than 2^31 rows");
-  SI_CHECK_ARG(table_width >= 0 && table_width <= (((int64_t)1 << 31) - 1 - kTile) / page_size,
+  SI_CHECK_ARG(table_width >= 0 && table_width <= (((int64_t)1 << 31) - 1 - 2 * kTile) / page_size,
                "si_paged_attn: page tables reach fewer than 2^31 positions");
   SI_CHECK_ARG(window >= 0 && window < ((int64_t)1 << 31), "si_paged_attn: bad window");
   SI_CHECK_ARG(group > 0 && D % group == 0, "si_paged_attn: group must divide D");
@@ -558,7 +1078,7 @@ extern "C" int si_paged_attn(const void* q, int q_dtype, int64_t B, int64_t Hq, 
   uintptr_t bits = 0;
   for (int j = 0; j < 4; ++j) {
     a.pool[j] = pool[j];
-    if (j < 2) bits |= reinterpret_cast<uintptr_t>(pool[j]);
+    bits |= reinterpret_cast<uintptr_t>(pool[j]);
   }
   a.sdt = dtype;
   a.out = out;
@@ -580,11 +1100,19 @@ extern "C" int si_paged_attn(const void* q, int q_dtype, int64_t B, int64_t Hq, 
                  need, workspace ? workspace_bytes : (size_t)0);
     a.parts = reinterpret_cast<float*>(workspace);
   }
+  if (q_dtype != SI_DT_F32) {
+    if (kind == kF16) return launch16<kF16, 1, 1>(a, deal, st);
+    if (kind == kBF16)
+      return q_dtype == SI_DT_BF16 ? launch16<kBF16, 1, 1>(a, deal, st) : launch16<kBF16, 2, 1>(a, deal, st);
+    if (kind == kI8) return launch16<kI8, 1, 1>(a, deal, st);
+    if (kind == kI4 && D / group <= 8)
+      return dtype == SI_DT_BF16 ? launch16<kI4, 1, 1>(a, deal, st) : launch16<kI4, 1, 2>(a, deal, st);
+  }
   switch (kind) {
-    case kF32: return launch_kind<kF32>(a, deal, st);
-    case kF16: return launch_kind<kF16>(a, deal, st);
-    case kBF16: return launch_kind<kBF16>(a, deal, st);
-    case kI8: return launch_kind<kI8>(a, deal, st);
-    default: return launch_kind<kI4>(a, deal, st);
+    case kF32: return launch32<kF32>(a, deal, st);
+    case kF16: return launch32<kF16>(a, deal, st);
+    case kBF16: return launch32<kBF16>(a, deal, st);
+    case kI8: return launch32<kI8>(a, deal, st);
+    default: return launch32<kI4>(a, deal, st);
   }
 }

@@ -190,7 +190,7 @@ def test_oracle_known_answers():
     k[1] = math.nan  # a page that only invalid entries could reach
     table = torch.tensor([[0, -1], [5, 0], [0, 0]], dtype=torch.int32)
     lengths = torch.tensor([4, 3, 0], dtype=torch.int32)
-    out, lse, _, _ = R.attend(q, k, v, table, lengths, 1.0)
+    out, lse, *_ = R.attend(q, k, v, table, lengths, 1.0)
     # positions 0, 1 of page 0 count, those of page -1 do not: weights 3/4, 1/4
     assert torch.allclose(out[0, 0], torch.tensor([3.0, 7.0], dtype=torch.float64))
     assert float(lse[0, 0]) == pytest.approx(math.log(4.0))
@@ -198,7 +198,7 @@ def test_oracle_known_answers():
     assert torch.allclose(out[1, 0], torch.tensor([4.0, 8.0], dtype=torch.float64))
     # no position: zeros and -inf
     assert (out[2] == 0).all() and float(lse[2, 0]) == -math.inf
-    out, _, _, _ = R.attend(q[:1], k, v, table[:1], torch.tensor([2], dtype=torch.int32), 1.0, window=1)
+    out, *_ = R.attend(q[:1], k, v, table[:1], torch.tensor([2], dtype=torch.int32), 1.0, window=1)
     assert torch.allclose(out[0, 0], torch.tensor([0.0, 4.0], dtype=torch.float64))
     x = torch.tensor([[[1.0, 0.0, 5.0]]])
     turned = R.rotate(x, torch.tensor([1]), torch.tensor([math.pi / 2], dtype=torch.float64), gain=2.0)

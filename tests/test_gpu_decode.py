@@ -410,13 +410,19 @@ def check_attention(q, pool, table, lengths, window=None, sm_scale=None):
     again = paged_attention(q, pool, table, lengths, sm_scale=sm_scale, window=window)
     assert np.array_equal(bits(again), bits(out))
     scale = 1 / math.sqrt(pool.head_dim) if sm_scale is None else sm_scale
-    want, wlse, weight, reach = R.attend(q, R.pool_values(pool, "k"), R.pool_values(pool, "v"), table, lengths,
+    want, wlse, weight, reach, peak = R.attend(q, R.pool_values(pool, "k"), R.pool_values(pool, "v"), table, lengths,
                                          scale, window)
     n = min(int(lengths.max()), table.shape[1] * pool.page_size) if lengths.numel() else 0
     slip = (pool.head_dim + 16) * U * (1 + reach)        # a score's error
     part = 2.0 ** -16 if q.dtype != F32 else 0.0
     rel = (2 * slip + (n / 4 + 64) * U + part)[..., None]
-    tol = rel * weight
+    # A weight p_t s_t (s_t: the factor of a quantized row, 1 of another) in two fp16 parts is
+    # scaled so that the largest of a row is 2^14 (2^13 at least where the scale is no power of two);
+    # fp16 steps by 2^-24 there, so each is off by 2^-25 at most, 2^-38 of the largest. Times the
+    # row's |v_td| / s_t, at most 128 for int8 and int4: 2^-38 n max_t(s_t p_t) 128, and s_t <= max |v_t|;
+    # for 16-bit rows 2^-38 n max_t(p_t) max |v|. It shows where the heaviest rows have a 0.
+    floor = 2.0 ** -38 * n * peak[..., None] if q.dtype != F32 else 0.0
+    tol = rel * weight + floor
     tol = tol + HALF_STEP[q.dtype] * (want.abs() + tol) + TINY[q.dtype]
     assert out.dtype == q.dtype and out.shape == q.shape and lse.dtype == F32
     nan = torch.isnan(want)  # a visible row may hold one
