@@ -653,7 +653,7 @@ int si_pool_read(const int64_t* slots, int64_t T, int64_t H, int64_t D, int64_t 
  * pool take no part), for t of the last `window` (0: all) of lengths[b] (int32, cut to
  * table_width * page_size) positions. Query head h reads kv head h / (Hq / Hk). out
  * [B, Hq, D] in q's dtype, lse [B, Hq] (natural logarithm; or NULL). No position:
- * out 0, lse -inf. D <= 512. The workspace (device, 4-byte aligned) may be 0 bytes
+ * out 0, lse -inf. D <= 512. The workspace (device, 16-byte aligned) may be 0 bytes
  * where the size query says so. */
 size_t si_paged_attn_workspace_bytes(int64_t Hq, int64_t Hk, int64_t D, int64_t capacity,
                                      int64_t window);

@@ -45,7 +45,7 @@ struct AttnArgs {
   int sdt;
   void* out;                // [B, Hk * group, D], q's type
   float* lse;               // [B, Hk * group] or NULL
-  float* parts;             // [2 * kParts][rows][D + 2], or NULL: one block per item
+  float* parts;             // [2 * kParts][part_rows][D], then [2 * kParts][part_rows][2]
   int part_rows;
 };
 
@@ -172,15 +172,15 @@ struct Engine32 {
   Running<J> st;
   float q[M * 8];
 
-  __device__ __forceinline__ void begin(const AttnArgs& a, int b, int64_t head0, int rows) {
+  // The item's query rows, from the block's LDS [kRows][DP + 4].
+  __device__ __forceinline__ void begin(const AttnArgs& a, const float (*rows)[DP + 4]) {
     const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
 #pragma unroll
     for (int m = 0; m < M; ++m) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = (m * 4 + kq) * 8 + e;
-        q[m * 8 + e] = c < rows && d < a.D
-                           ? load_any(a.q, a.qdt, b * a.qs[0] + (head0 + c) * a.qs[1] + d) : 0.0f;
+      for (int e = 0; e < 8; e += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(&rows[c][(m * 4 + kq) * 8 + e]);
+        q[m * 8 + e] = x.x; q[m * 8 + e + 1] = x.y; q[m * 8 + e + 2] = x.z; q[m * 8 + e + 3] = x.w;
       }
     }
   }
@@ -308,6 +308,17 @@ __device__ __forceinline__ h2 as_h2(uint32_t u) { return __builtin_bit_cast(h2, 
 __device__ __forceinline__ uint32_t as_u32(h2 h) { return __builtin_bit_cast(uint32_t, h); }
 __device__ __forceinline__ h2 pair(float x) { return h2{(_Float16)x, (_Float16)x}; }
 
+// Two nibbles of a word, at bits 0 and 16 (HIGH: 4 and 20), as fp16 values n - 8. The
+// constants are kept in registers, where one v_and_or_b32 can take both.
+template <bool HIGH>
+__device__ __forceinline__ h2 nibbles(uint32_t u) {
+  uint32_t mask = HIGH ? 0x00f000f0u : 0x000f000fu, base = 0x64006400u;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(base));
+  const h2 x = as_h2((u & mask) | base);  // 1024 + n, or 1024 + 16 n
+  return HIGH ? __builtin_elementwise_fma(x, pair(0.0625f), pair(-72.0f)) : x - pair(1032.0f);
+}
+
 template <int WORDS>
 __device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
   if constexpr (WORDS == 0) {
@@ -364,18 +375,19 @@ struct Engine16 {
     return (m * 4 + kq) * 8;
   }
 
-  __device__ __forceinline__ void begin(const AttnArgs& a, int b, int64_t head0, int rows) {
+  __device__ __forceinline__ void begin(const AttnArgs& a, const float (*rows)[DP + 4]) {
     const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
     float x[M][8];
     float top = 0.0f;
 #pragma unroll
     for (int m = 0; m < M; ++m) {
+      const f32x4 u = *reinterpret_cast<const f32x4*>(&rows[c][chunk_d(m, kq)]);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(&rows[c][chunk_d(m, kq) + 4]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         constexpr int order[8] = {1, 5, 0, 4, 3, 7, 2, 6};
-        const int d = chunk_d(m, kq) + (KIND == kI4 ? order[e] : e);
-        x[m][e] = c < rows && d < a.D
-                      ? load_any(a.q, a.qdt, b * a.qs[0] + (head0 + c) * a.qs[1] + d) : 0.0f;
+        const int n = KIND == kI4 ? order[e] : e;
+        x[m][e] = n < 4 ? u[n & 3] : v[n & 3];
         top = fmaxf(top, fabsf(x[m][e]));
       }
     }
@@ -559,10 +571,10 @@ struct Engine16 {
       }
     } else {
       const uint32_t u = x.k[s][m], w = u >> 8;
-      r[0] = as_u32((as_h2((u & 0x000f000fu) | 0x64006400u) - pair(1032.0f)) * scale);
-      r[1] = as_u32((as_h2((u & 0x00f000f0u) | 0x64006400u) * pair(0.0625f) - pair(72.0f)) * scale);
-      r[2] = as_u32((as_h2((w & 0x000f000fu) | 0x64006400u) - pair(1032.0f)) * scale);
-      r[3] = as_u32((as_h2((w & 0x00f000f0u) | 0x64006400u) * pair(0.0625f) - pair(72.0f)) * scale);
+      r[0] = as_u32(nibbles<false>(u) * scale);
+      r[1] = as_u32(nibbles<true>(u) * scale);
+      r[2] = as_u32(nibbles<false>(w) * scale);
+      r[3] = as_u32(nibbles<true>(w) * scale);
     }
     return r;
   }
@@ -582,8 +594,8 @@ struct Engine16 {
       out[3] = as_u32(as_h2(__builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u)) - pair(1152.0f));
     } else {  // byte i: values 2i (high nibble) and 2i + 1
       const uint32_t u = __builtin_amdgcn_perm(b[0], a[0], 0x0c040c00u + 0x00010001u * i);
-      out[0] = as_u32(as_h2((u & 0x00f000f0u) | 0x64006400u) * pair(0.0625f) - pair(72.0f));
-      out[1] = as_u32(as_h2((u & 0x000f000fu) | 0x64006400u) - pair(1032.0f));
+      out[0] = as_u32(nibbles<true>(u));
+      out[1] = as_u32(nibbles<false>(u));
     }
   }
 
@@ -663,14 +675,16 @@ struct Engine16 {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float u = w[2 * i], v = w[2 * i + 1];
-      if constexpr (kBf) {
-        hi[i] = f32x2_to_bf16x2_bits(u, v);
-        lo[i] = f32x2_to_bf16x2_bits(u - __uint_as_float(hi[i] << 16), v - __uint_as_float(hi[i] & 0xffff0000u));
-      } else {
-        const h2 h = {(_Float16)u, (_Float16)v};
-        hi[i] = as_u32(h);
-        lo[i] = as_u32(h2{(_Float16)(u - (float)h.x), (_Float16)(v - (float)h.y)});
-      }
+      // The bits that lo completes are the operand's own: left to itself the compiler
+      // takes them from e * sv rounded once, which differs where the product's fp32
+      // rounding lies halfway between two fp16 values.
+      uint32_t h = kBf ? f32x2_to_bf16x2_bits(u, v) : as_u32(h2{(_Float16)u, (_Float16)v});
+      asm("" : "+v"(h));
+      hi[i] = h;
+      if constexpr (kBf)
+        lo[i] = f32x2_to_bf16x2_bits(u - __uint_as_float(h << 16), v - __uint_as_float(h & 0xffff0000u));
+      else
+        lo[i] = as_u32(h2{(_Float16)(u - (float)as_h2(h).x), (_Float16)(v - (float)as_h2(h).y)});
     }
 
     uint2 vs[NS][2];
@@ -748,6 +762,11 @@ struct Engine16 {
   static constexpr float kRoom = 14.0f;
 };
 
+// The maximum and sum of partial row i (slot * part_rows + row) at 2 i.
+__device__ __forceinline__ float* part_sums(const AttnArgs& a) {
+  return a.parts + (int64_t)2 * kParts * a.part_rows * a.D;
+}
+
 // DEALT: tiles dealt evenly to kParts blocks, partial results in a.parts. Otherwise
 // block = item, which it finishes.
 template <class E, bool DEALT>
@@ -809,13 +828,20 @@ __global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
     const int rows = a.group - rb * kRows < kRows ? a.group - rb * kRows : kRows;
     const int64_t head0 = (int64_t)hk * a.group + rb * kRows;
 
+    // the item's query rows in fp32, zeros behind them
+    for (int x = tid; x < kRows * DP; x += 256) {
+      const int r = x / DP, d = x - r * DP;
+      lds_o[0][r][d] = r < rows && d < a.D ? load_any(a.q, a.qdt, b * a.qs[0] + (head0 + r) * a.qs[1] + d) : 0.0f;
+    }
+    __syncthreads();
     E e;
     Running<J>& st = e.st;
     st.m = -INFINITY;
     st.l = 0.0f;
 #pragma unroll
     for (int j = 0; j < J; ++j) st.o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    e.begin(a, b, head0, rows);
+    e.begin(a, lds_o[0]);
+    if (E::kLds) __syncthreads();  // the waves' own memory lies there too
     e.walk(a, lds + wave * E::kLds, b, hk, lo, hi, ta, tb);
 
     // the four waves' results together
@@ -852,12 +878,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
         store_any(a.out, a.qdt, o * a.D + d, sum == 0.0f ? 0.0f : val / sum);
         if (d == 0 && a.lse) a.lse[o] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
       } else {
-        float* part = a.parts + (slot * a.part_rows + r) * (a.D + 2);
-        part[d] = val;
-        if (d == 0) {
-          part[a.D] = top;
-          part[a.D + 1] = sum;
-        }
+        const int64_t at = slot * a.part_rows + r;
+        a.parts[at * a.D + d] = val;
+        if (d == 0) *reinterpret_cast<float2*>(part_sums(a) + 2 * at) = make_float2(top, sum);
       }
     }
     if (!DEALT) return;
@@ -873,16 +896,22 @@ __global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
 }
 
 // Joins the partial results of items that several blocks worked on, and gives the
-// items without positions their zeros. Block (x, y): row y of item x, a thread a value.
+// items without positions their zeros. Block (x, y): row y of item x. The maxima
+// and sums of all parts come first, in one round of loads; then D / 4 threads take
+// four values each of every (1024 / D)-th part.
 __global__ __launch_bounds__(256) void paged_join(AttnArgs a) {
   __shared__ int64_t lds_scan[8];
+  __shared__ float weight[kParts];
+  __shared__ f32x4 lds_o[256];
+  __shared__ float red[8];
+  const int tid = threadIdx.x;
   const int per = a.Hk * a.rb;
   const int b = blockIdx.x / per, item = blockIdx.x - b * per;
   const int hk = item / a.rb, rb = item - hk * a.rb;
   const int r = blockIdx.y;
   int64_t total_mine = 0, before_mine = 0;
   int32_t lo, hi;
-  for (int i = threadIdx.x; i < a.B; i += blockDim.x) {
+  for (int i = tid; i < a.B; i += 256) {
     const int64_t n = (int64_t)span_tiles(a, i, &lo, &hi) * per;
     total_mine += n;
     if (i < b) before_mine += n;
@@ -894,28 +923,64 @@ __global__ __launch_bounds__(256) void paged_join(AttnArgs a) {
   const int n = span_tiles(a, b, &lo, &hi);
   const int64_t head = (int64_t)hk * a.group + rb * kRows + r;
   const int64_t o = (int64_t)b * a.Hk * a.group + head;
-  const int d = threadIdx.x;
   if (n == 0) {
-    if (d < a.D) store_any(a.out, a.qdt, o * a.D + d, 0.0f);
-    if (d == 0 && a.lse) a.lse[o] = -INFINITY;
+    if (tid < a.D) store_any(a.out, a.qdt, o * a.D + tid, 0.0f);
+    if (tid == 0 && a.lse) a.lse[o] = -INFINITY;
     return;
   }
   const int64_t f0 = before + (int64_t)item * n, parts = si_part_count(total, kParts);
-  const int64_t w0 = si_part_of(f0, total, parts), w1 = si_part_of(f0 + n - 1, total, parts);
-  if (w0 == w1) return;  // its block finished it
-  float top = -INFINITY, sum = 0.0f, val = 0.0f;
-  for (int64_t w = w0; w <= w1; ++w) {
-    const bool inside = si_part_begin(w, total, parts) > f0;
-    const float* part = a.parts + (si_part_slot(w, inside) * a.part_rows + r) * (a.D + 2);
-    const float m = part[a.D], l = part[a.D + 1], x = d < a.D ? part[d] : 0.0f;
-    const float up = fmaxf(top, m), ref = up == -INFINITY ? 0.0f : up;
-    const float k0 = __builtin_amdgcn_exp2f(top - ref), k1 = __builtin_amdgcn_exp2f(m - ref);
-    sum = sum * k0 + l * k1;
-    val = val * k0 + x * k1;
-    top = up;
+  const int64_t w0 = si_part_of(f0, total, parts);
+  const int count = (int)(si_part_of(f0 + n - 1, total, parts) - w0) + 1;
+  if (count == 1) return;  // its block finished it
+  // of every part: its slot is 2 w but for the first, whose block began with the item or before
+  const bool inside = si_part_begin(w0, total, parts) > f0;
+  auto row = [&](int i) { return si_part_slot(w0 + i, i > 0 || inside) * a.part_rows + r; };
+  float m[kParts / 256], l[kParts / 256], top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kParts / 256; ++i) {
+    const int w = tid + 256 * i;
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+    if (w < count) {
+      const float2 x = *reinterpret_cast<const float2*>(part_sums(a) + 2 * row(w));
+      m[i] = x.x;
+      l[i] = x.y;
+    }
+    top = fmaxf(top, m[i]);
   }
-  if (d < a.D) store_any(a.out, a.qdt, o * a.D + d, sum == 0.0f ? 0.0f : val / sum);
-  if (d == 0 && a.lse) a.lse[o] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kParts / 256; ++i) {
+    const float k = __builtin_amdgcn_exp2f(m[i] - ref);
+    weight[tid + 256 * i] = k;
+    sum += l[i] * k;
+  }
+  for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x, 64);
+  if ((tid & 63) == 0) red[4 + (tid >> 6)] = sum;
+  __syncthreads();
+  sum = (red[4] + red[5]) + (red[6] + red[7]);
+  const int width = a.D / 4, lanes = 256 / width;  // lanes: parts at a time
+  const int d4 = tid % width, g = tid / width;
+  f32x4 val = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (g < lanes) {
+#pragma unroll 4
+    for (int w = g; w < count; w += lanes)
+      val += *reinterpret_cast<const f32x4*>(a.parts + row(w) * a.D + 4 * d4) * weight[w];
+  }
+  lds_o[tid] = val;
+  __syncthreads();
+  if (tid < width) {
+    for (int i = 1; i < lanes; ++i) val += lds_o[tid + i * width];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      store_any(a.out, a.qdt, o * a.D + 4 * tid + j, sum == 0.0f ? 0.0f : val[j] / sum);
+    if (tid == 0 && a.lse) a.lse[o] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  }
 }
 
 // Any head size and group: block = (sequence, query head), a thread a position of
@@ -1001,7 +1066,7 @@ int launch(const AttnArgs& a, bool deal, hipStream_t st) {
   if (deal) {
     paged_attn<E, true><<<kParts, 256, 0, st>>>(a);
     const int rows = a.group < kRows ? a.group : kRows;
-    paged_join<<<dim3((unsigned)items, (unsigned)rows), a.D <= 64 ? 64 : 128, 0, st>>>(a);
+    paged_join<<<dim3((unsigned)items, (unsigned)rows), 256, 0, st>>>(a);
   } else {
     paged_attn<E, false><<<(unsigned)items, 256, 0, st>>>(a);
   }
@@ -1098,6 +1163,7 @@ extern "C" int si_paged_attn(const void* q, int q_dtype, int64_t B, int64_t Hq, 
     const size_t need = si_paged_attn_workspace_bytes(Hq, Hk, D, a.capacity, window);
     SI_CHECK_ARG(workspace && workspace_bytes >= need, "si_paged_attn: workspace of %zu bytes needed, got %zu",
                  need, workspace ? workspace_bytes : (size_t)0);
+    SI_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "si_paged_attn: workspace not 16-byte aligned");
     a.parts = reinterpret_cast<float*>(workspace);
   }
   if (q_dtype != SI_DT_F32) {

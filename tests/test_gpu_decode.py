@@ -500,7 +500,7 @@ def test_attention_long_and_uneven(lens, dtype):
 def test_attention_many_sequences():
     """More sequences than a block has threads."""
     g = gen(11)
-    lens = torch.randint(0, 60, (700,)).tolist()
+    lens = torch.randint(0, 60, (700,), generator=torch.Generator().manual_seed(131)).tolist()
     lens[3], lens[650] = 900, 450
     pool, table, lengths = make_cache(g, lens, 1, 64, 16, "int8", BF16)
     check_attention(randn(g, 700, 2, 64, dtype=BF16), pool, table, lengths)
@@ -594,6 +594,32 @@ def test_attention_nan_in_a_visible_row(precision, dtype):
         # the same row behind the sequence's end does nothing
         lengths[0] = 4 * 16 + 3
         assert torch.isfinite(paged_attention(q, pool, table, lengths)).all()
+
+
+@pytest.mark.parametrize("qt,dtype,precision,part", [(F16, F16, "fp32", 2.0 ** -21), (BF16, BF16, "int8", 2.0 ** -21),
+                                                     (BF16, F32, "int8", 2.0 ** -21), (BF16, BF16, "int4", 2.0 ** -21),
+                                                     (F16, F16, "int4", 2.0 ** -19), (BF16, BF16, "fp32", 2.0 ** -15)])
+def test_attention_weights_keep_both_parts(qt, dtype, precision, part):
+    """Two-part weights are 2^-22 (fp16) or 2^-16 (bf16) exact for every single one of many: where a row's
+    values cancel, a weight that lost its low part (2^-12) would show. (int4 with fp16 scales: its
+    scales are in two parts as well, 2^-20.)"""
+    g = gen(23)
+    B, n, H, D = 6000, 6, 2, 64
+    pool = KVPagePool(B, 1, D, page_size=8, precision=precision, dtype=dtype)
+    k, v = randn(g, B * n, 1, D, dtype=dtype), randn(g, B * n, 1, D, dtype=dtype)
+    at = torch.arange(B * n, device="cuda")
+    pool.write(k, v, at // n * 8 + at % n)
+    q = randn(g, B, H, D, dtype=qt)
+    table = torch.arange(B, dtype=torch.int32, device="cuda")[:, None]
+    out = paged_attention(q, pool, table, torch.full((B,), n, dtype=torch.int32, device="cuda")).double()
+    kk, vv = (R.pool_values(pool, x)[:, 0, :n] for x in ("k", "v"))          # [B, n, D]
+    s = torch.matmul(q.double(), kk.transpose(1, 2).contiguous()) / math.sqrt(D)
+    p = torch.softmax(s, -1)
+    want, weight = torch.matmul(p, vv), torch.matmul(p, vv.abs())
+    slip = (D + 16) * U * (1 + s.abs().amax(-1, keepdim=True) * 8)
+    tol = (2 * slip + 80 * U + part) * weight
+    tol = tol + HALF_STEP[qt] * (want.abs() + tol) + TINY[qt]
+    assert ((out - want).abs() <= tol).all(), float(((out - want).abs() / tol).max())
 
 
 def test_attention_strides_and_scale():
