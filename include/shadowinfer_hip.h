@@ -600,7 +600,18 @@ int si_reuse_apply(const void* hidden, const void* hidden_in, const void* hidden
                    int64_t n, void* out, si_stream_t stream);
 
 /* Serving-side operators (no reference counterpart): rotary positions, a page
- * pool of many sequences, and attention of one new token over it. */
+ * pool of many sequences, and attention of one new token over it. Their structs are
+ * host memory, read before the call returns. */
+
+/* A rotation: pair i of a token at position p turns by p * freq[i] turns of 2 pi
+ * (device double [pairs]) and is scaled by gain. Pairs are (i, i + pairs), or (2i,
+ * 2i + 1) with interleaved. Angles in 64 bits, products in fp32, one rounding. */
+typedef struct {
+  int64_t pairs;
+  int64_t interleaved;
+  const double* freq;
+  double gain;
+} si_rotation;
 
 /* Rows of one tensor [B, S, heads, D] of a rotary call: element strides of
  * batches, tokens and heads; the values of a head are contiguous. dst may be src
@@ -613,56 +624,59 @@ typedef struct {
   int64_t dst_stride[3];
 } si_rotary_rows;
 
-/* Rotary positions of q and (unless NULL) k, structs on the host: pair i of a
- * token at position p turns by p * freq[i] turns of 2 pi (device double [pairs])
- * and is scaled by gain; transpose turns the other way. Pairs are (i, i + pairs),
- * or (2i, 2i + 1) with interleaved; values from 2 * pairs on are copied. positions:
- * int64 (positions64) or int32, element (b, s) at b * pos_stride_b + s *
- * pos_stride_s, any value. Angles in 64 bits, products in fp32, one rounding. D <= 1024. */
-int si_rotary(const si_rotary_rows* q, const si_rotary_rows* k, int dtype, int64_t B, int64_t S,
-              int64_t D, int64_t pairs, int interleaved, const double* freq, double gain,
-              int transpose, const void* positions, int positions64, int64_t pos_stride_b,
-              int64_t pos_stride_s, si_stream_t stream);
+/* Rotary positions of q and (unless NULL) k; transpose turns the other way. Values
+ * from 2 * pairs on are copied. positions: int64 (positions64) or int32, element (b,
+ * s) at b * pos_stride_b + s * pos_stride_s, any value. D <= 1024. */
+int si_rotary(const si_rotation* rotation, const si_rotary_rows* q, const si_rotary_rows* k, int dtype,
+              int64_t B, int64_t S, int64_t D, int transpose, const void* positions, int positions64,
+              int64_t pos_stride_b, int64_t pos_stride_s, si_stream_t stream);
 
-/* Page pool (KVPagePool): tensors k, v [pages, H, page_size, row] and, for int8 /
- * int4, scale_k, scale_v [pages, H, page_size, 1 or D / group] in the pool's dtype,
- * rows as in the paged store (`pool`: host array of these 4 device pointers). Fewer
- * than 2^31 rows, D <= 1024.
- *
- * Write: K and V [T, H, D] (element strides of tokens and heads, values of a head
- * contiguous) of token t to slot slots[t] = page * page_size + offset (int64); a
- * slot outside the pool is skipped, and no slot comes twice in a call. With pairs > 0
- * K is rotated first as by si_rotary (position t at t * pos_stride) and rounded to
- * its dtype. */
-int si_pool_write(const void* k, const void* v, int dtype, int64_t T, int64_t H, int64_t D,
+/* A page pool (KVPagePool): tensors k, v [pages, heads, page_size, row] and, for int8 /
+ * int4, scale_k, scale_v [pages, heads, page_size, 1 or D / group] in the pool's
+ * dtype, rows as in the paged store. 16-byte aligned, fewer than 2^31 rows, D <= 512. */
+typedef struct {
+  int64_t pages;
+  int64_t heads;
+  int64_t page_size;
+  int64_t D;
+  int64_t precision;
+  int64_t dtype;
+  int64_t group;
+  void* k;
+  void* v;
+  void* scale_k;
+  void* scale_v;
+} si_page_pool;
+
+/* Write: K and V [T, heads, D] in the pool's dtype (element strides of tokens and
+ * heads, values of a head contiguous) of token t to slot slots[t] = page * page_size +
+ * offset (int64); a slot outside the pool is skipped, and no slot comes twice in a
+ * call. With a rotation (or NULL) K is rotated first as by si_rotary (position t at
+ * t * pos_stride) and rounded to its dtype. */
+int si_pool_write(const si_page_pool* pool, const void* k, const void* v, int64_t T,
                   int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
-                  const int64_t* slots, int64_t pages, int64_t page_size, int precision,
-                  int64_t group, void* const* pool, int64_t pairs, int interleaved,
-                  const double* freq, double gain, const void* positions, int positions64,
-                  int64_t pos_stride, si_stream_t stream);
+                  const int64_t* slots, const si_rotation* rotation, const void* positions,
+                  int positions64, int64_t pos_stride, si_stream_t stream);
 
-/* Read: the values of slots[t] into out_k, out_v [T, H, D] in out_dtype; zeros for a
- * slot outside the pool. dtype is the pool's. */
-int si_pool_read(const int64_t* slots, int64_t T, int64_t H, int64_t D, int64_t pages,
-                 int64_t page_size, int precision, int dtype, int64_t group, void* const* pool,
-                 void* out_k, void* out_v, int out_dtype, si_stream_t stream);
+/* Read: the values of slots[t] into out_k, out_v [T, heads, D] in out_dtype; zeros for
+ * a slot outside the pool. */
+int si_pool_read(const si_page_pool* pool, const int64_t* slots, int64_t T, void* out_k, void* out_v,
+                 int out_dtype, si_stream_t stream);
 
 /* Attention of one token of each sequence, q [B, Hq, D] (element strides of
  * sequences and heads), over the pool's rows: position t of sequence b is in page
  * table[b * table_stride + t / page_size] (int32; positions of a page outside the
  * pool take no part), for t of the last `window` (0: all) of lengths[b] (int32, cut to
- * table_width * page_size) positions. Query head h reads kv head h / (Hq / Hk). out
+ * table_width * page_size) positions. Query head h reads kv head h / (Hq / heads). out
  * [B, Hq, D] in q's dtype, lse [B, Hq] (natural logarithm; or NULL). No position:
- * out 0, lse -inf. D <= 512. The workspace (device, 16-byte aligned) may be 0 bytes
- * where the size query says so. */
-size_t si_paged_attn_workspace_bytes(int64_t Hq, int64_t Hk, int64_t D, int64_t capacity,
+ * out 0, lse -inf. The workspace (device, 16-byte aligned; capacity = table_width *
+ * page_size) may be 0 bytes where the size query says so. */
+size_t si_paged_attn_workspace_bytes(int64_t Hq, int64_t heads, int64_t D, int64_t capacity,
                                      int64_t window);
-int si_paged_attn(const void* q, int q_dtype, int64_t B, int64_t Hq, int64_t q_stride_b,
-                  int64_t q_stride_h, int64_t Hk, int64_t D, const int32_t* table,
-                  int64_t table_stride, int64_t table_width, const int32_t* lengths, int64_t window,
-                  float scale, int64_t pages, int64_t page_size, int precision, int dtype,
-                  int64_t group, void* const* pool, void* out, float* lse, void* workspace,
-                  size_t workspace_bytes, si_stream_t stream);
+int si_paged_attn(const si_page_pool* pool, const void* q, int q_dtype, int64_t B, int64_t Hq,
+                  int64_t q_stride_b, int64_t q_stride_h, const int32_t* table, int64_t table_stride,
+                  int64_t table_width, const int32_t* lengths, int64_t window, float scale, void* out,
+                  float* lse, void* workspace, size_t workspace_bytes, si_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,7 @@
 // lie inside its range, and leaves the maximum, sum and unnormalised output of the
 // at most two that go over its edges in the workspace, where paged_join merges them.
 // The lengths are read on the device, so a captured graph replays with new ones.
+#include "si_pool_args.h"
 #include "si_pool_index.h"
 #include "si_kv_common.h"
 
@@ -23,7 +24,8 @@ namespace {
 constexpr int kRows = 16;        // query heads of an item
 constexpr int kWaveTokens = 32;
 constexpr int kTile = 4 * kWaveTokens;
-constexpr int kParts = 512;      // workgroups of a dealt launch: two per CU
+constexpr int kCUs = 256;
+constexpr int kMostParts = 4 * kCUs;  // workgroups of a dealt launch at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -45,7 +47,8 @@ struct AttnArgs {
   int sdt;
   void* out;                // [B, Hk * group, D], q's type
   float* lse;               // [B, Hk * group] or NULL
-  float* parts;             // [2 * kParts][part_rows][D], then [2 * kParts][part_rows][2]
+  int most;                 // workgroups of a dealt launch
+  float* parts;             // [2 * most][part_rows][D], then [2 * most][part_rows][2]
   int part_rows;
 };
 
@@ -169,6 +172,7 @@ __device__ __forceinline__ float max_over_kq(float v) {
 template <int KIND, int DP_>
 struct Engine32 {
   static constexpr int DP = DP_, J = DP / 16, M = DP / 32, kLds = 0;
+  static constexpr int kBlocks = 4;  // of a CU, for the registers' bound and the dealing
   Running<J> st;
   float q[M * 8];
 
@@ -296,8 +300,9 @@ struct Engine32 {
 // The k order within a chunk of eight is free as long as both operands have the
 // same: int4's nibbles come out as 1 5 0 4 3 7 2 6.
 //
-// HBM bounds it: each wave has the next tile's rows in flight while it works on
-// one (two register buffers), rows and scales of a tile go through LDS.
+// HBM bounds it: a wave has the next tile's keys in flight during the softmax and
+// the second product, and its values during the first; rows and scales of a tile go
+// through LDS.
 // ---------------------------------------------------------------------------
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -342,6 +347,8 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t* w) {
 template <int KIND, int DP_, bool EXACT, int NQ, int NS>
 struct Engine16 {
   static constexpr int DP = DP_, J = DP / 16, M = DP / 32;
+  // Blocks of a CU, for the registers' bound and the dealing.
+  static constexpr int kBlocks = KIND == kI8 || KIND == kI4 ? 3 : 2;
   static constexpr bool kBf = KIND == kBF16;
   static constexpr bool kScaled = KIND == kI8 || KIND == kI4;
   static constexpr int kG = 8;  // int4 groups of a row at most
@@ -351,9 +358,9 @@ struct Engine16 {
   static constexpr int kVW1 = kVW ? kVW : 1;
   static constexpr int kUnit = 8 * kBits / 32;  // words of eight values
 
-  // A wave's LDS: rows [2][32], then per position: K's factor, V's factor, its
+  // A wave's LDS: rows [32], then per position: K's factor, V's factor, its
   // logarithm, and int4's s' as [32][kG] for K and [kG][32] for V, NS parts each.
-  static constexpr int kLdsScale = 2 * 32 * 4;
+  static constexpr int kLdsScale = 32 * 4;
   static constexpr int kLdsParts = kLdsScale + (kScaled ? 3 * 32 * 4 : 0);
   static constexpr int kLds = kLdsParts + (KIND == kI4 ? 2 * NS * 32 * kG * 2 : 0);
 
@@ -425,16 +432,16 @@ struct Engine16 {
     return t < hi ? a.table[b * a.ts + (uint32_t)t / (uint32_t)a.P] : -1;
   }
 
-  // Starts the loads of a tile. Positions that do not take part read row 0.
-  __device__ __forceinline__ static void start(const AttnArgs& a, int32_t* lds_rows, int hk, int32_t t0,
-                                               int32_t hi, int32_t page, Tile& x) {
+  // Starts the loads of a tile's keys and scales, its rows into LDS. Positions that do
+  // not take part read row 0.
+  __device__ __forceinline__ static void start_keys(const AttnArgs& a, int32_t* lds_rows, int hk, int32_t t0,
+                                                    int32_t hi, int32_t page, Tile& x) {
     const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
     const int32_t t = t0 + (lane & 31);
     x.row = t < hi ? si_page_row(page, a.pages, hk, a.Hk, (int32_t)((uint32_t)t % (uint32_t)a.P), a.P) : -1;
     if (lane < 32) lds_rows[lane] = x.row;
     wave_sync();
     const char* kp = reinterpret_cast<const char*>(a.pool[0]);
-    const char* vp = reinterpret_cast<const char*>(a.pool[1]);
     const int64_t row_bytes = (int64_t)a.D * kBits / 8;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -464,24 +471,6 @@ struct Engine16 {
         }
       }
     }
-    x.live = 0;
-    const bool in = EXACT || c * J < a.D;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int4 r4 = *reinterpret_cast<const int4*>(lds_rows + s * 16 + kq * 4);
-      const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (r[i] >= 0) x.live |= 1u << (4 * s + i);
-        const char* p = vp + (r[i] < 0 ? 0 : r[i]) * row_bytes + c * J * kBits / 8;
-        if (in) {
-          load_words<kVW>(p, x.v[s][i]);
-        } else {
-#pragma unroll
-          for (int w = 0; w < kVW1; ++w) x.v[s][i][w] = KIND == kI4 ? 0x88888888u : 0u;
-        }
-      }
-    }
     if constexpr (kScaled) {  // K's scales in the lower lanes, V's in the upper
       const int64_t r = x.row < 0 ? 0 : x.row;
       const void* sp = a.pool[lane < 32 ? 2 : 3];
@@ -508,6 +497,31 @@ struct Engine16 {
             else if (a.sdt == SI_DT_F32) x.sc[w] = reinterpret_cast<const uint32_t*>(sp)[r * G + w];
             else x.sc[w] = __float_as_uint(load_any(sp, a.sdt, r * G + w));
           }
+        }
+      }
+    }
+  }
+
+  // Starts the loads of its values; which of the lane's positions take part.
+  __device__ __forceinline__ static void start_values(const AttnArgs& a, const int32_t* lds_rows, Tile& x) {
+    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
+    const char* vp = reinterpret_cast<const char*>(a.pool[1]);
+    const int64_t row_bytes = (int64_t)a.D * kBits / 8;
+    x.live = 0;
+    const bool in = EXACT || c * J < a.D;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int4 r4 = *reinterpret_cast<const int4*>(lds_rows + s * 16 + kq * 4);
+      const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r[i] >= 0) x.live |= 1u << (4 * s + i);
+        const char* p = vp + (r[i] < 0 ? 0 : r[i]) * row_bytes + c * J * kBits / 8;
+        if (in) {
+          load_words<kVW>(p, x.v[s][i]);
+        } else {
+#pragma unroll
+          for (int w = 0; w < kVW1; ++w) x.v[s][i][w] = KIND == kI4 ? 0x88888888u : 0u;
         }
       }
     }
@@ -606,14 +620,12 @@ struct Engine16 {
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), z, 0, 0, 0);
   }
 
-  __device__ __forceinline__ void work(const AttnArgs& a, char* lds, const Tile& x) {
+  // The scores of a tile, without their factors.
+  __device__ __forceinline__ void scores(const AttnArgs& a, char* lds, const Tile& x, f32x4* acc) {
     const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
-    const float* factor = reinterpret_cast<const float*>(lds + kLdsScale);
     const _Float16* kpart = reinterpret_cast<const _Float16*>(lds + kLdsParts);
-    const _Float16* vpart = kpart + NS * 32 * kG;
     if constexpr (kScaled) place_scales(a, lds, x);
-
-    f32x4 acc[2] = {};
+    acc[0] = acc[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -633,7 +645,13 @@ struct Engine16 {
         }
       }
     }
+  }
 
+  // Its weights and their products with the values.
+  __device__ __forceinline__ void values(const AttnArgs& a, const char* lds, const Tile& x, const f32x4* acc) {
+    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
+    const float* factor = reinterpret_cast<const float*>(lds + kLdsScale);
+    const _Float16* vpart = reinterpret_cast<const _Float16*>(lds + kLdsParts) + NS * 32 * kG;
     float w[8], y[8], top = st.m;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -737,24 +755,23 @@ struct Engine16 {
     const int32_t end = tb * (int64_t)kTile + lo < hi ? lo + tb * kTile : hi;
     if (t0 >= end) return;
     int32_t* rows = reinterpret_cast<int32_t*>(lds);
-    Tile x, z;
-    start(a, rows, hk, t0, hi, entry(a, b, t0, hi), x);
+    Tile x;
+    f32x4 acc[2];
+    start_keys(a, rows, hk, t0, hi, entry(a, b, t0, hi), x);
+    start_values(a, rows, x);
     int32_t page = entry(a, b, t0 + kTile, hi);
+    // a tile's keys are loaded over the last one's once its scores are done, its values
+    // once its products are
     while (true) {
+      scores(a, lds, x, acc);
       t0 += kTile;
       if (t0 < end) {
-        start(a, rows + 32, hk, t0, hi, page, z);
+        start_keys(a, rows, hk, t0, hi, page, x);
         page = entry(a, b, t0 + kTile, hi);
       }
-      work(a, lds, x);
+      values(a, lds, x, acc);
       if (t0 >= end) break;
-      t0 += kTile;
-      if (t0 < end) {
-        start(a, rows, hk, t0, hi, page, x);
-        page = entry(a, b, t0 + kTile, hi);
-      }
-      work(a, lds, z);
-      if (t0 >= end) break;
+      start_values(a, rows, x);
     }
     // the sums above are of weights scaled by 2^kRoom
     st.m -= kRoom;
@@ -764,13 +781,13 @@ struct Engine16 {
 
 // The maximum and sum of partial row i (slot * part_rows + row) at 2 i.
 __device__ __forceinline__ float* part_sums(const AttnArgs& a) {
-  return a.parts + (int64_t)2 * kParts * a.part_rows * a.D;
+  return a.parts + (int64_t)2 * a.most * a.part_rows * a.D;
 }
 
-// DEALT: tiles dealt evenly to kParts blocks, partial results in a.parts. Otherwise
+// DEALT: tiles dealt evenly to a.most blocks, partial results in a.parts. Otherwise
 // block = item, which it finishes.
 template <class E, bool DEALT>
-__global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
+__global__ __launch_bounds__(256, E::kBlocks) void paged_attn(AttnArgs a) {
   constexpr int DP = E::DP, J = DP / 16;
   // the waves' own memory while they walk, their outputs afterwards
   constexpr int kOut = kRows * (DP + 4) * (int)sizeof(float);
@@ -794,7 +811,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
     for (int i = b0; i < b1; ++i) mine += (int64_t)span_tiles(a, i, &lo, &hi) * per;
     int64_t before;
     total = block_scan(mine, lds_scan, &before);
-    const int64_t parts = si_part_count(total, kParts);
+    const int64_t parts = si_part_count(total, a.most);
     if (blockIdx.x >= parts) return;
     f = si_part_begin(blockIdx.x, total, parts);
     end = si_part_begin(blockIdx.x + 1, total, parts);
@@ -901,7 +918,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn(AttnArgs a) {
 // four values each of every (1024 / D)-th part.
 __global__ __launch_bounds__(256) void paged_join(AttnArgs a) {
   __shared__ int64_t lds_scan[8];
-  __shared__ float weight[kParts];
+  __shared__ float weight[kMostParts];
   __shared__ f32x4 lds_o[256];
   __shared__ float red[8];
   const int tid = threadIdx.x;
@@ -928,16 +945,16 @@ __global__ __launch_bounds__(256) void paged_join(AttnArgs a) {
     if (tid == 0 && a.lse) a.lse[o] = -INFINITY;
     return;
   }
-  const int64_t f0 = before + (int64_t)item * n, parts = si_part_count(total, kParts);
+  const int64_t f0 = before + (int64_t)item * n, parts = si_part_count(total, a.most);
   const int64_t w0 = si_part_of(f0, total, parts);
   const int count = (int)(si_part_of(f0 + n - 1, total, parts) - w0) + 1;
   if (count == 1) return;  // its block finished it
   // of every part: its slot is 2 w but for the first, whose block began with the item or before
   const bool inside = si_part_begin(w0, total, parts) > f0;
   auto row = [&](int i) { return si_part_slot(w0 + i, i > 0 || inside) * a.part_rows + r; };
-  float m[kParts / 256], l[kParts / 256], top = -INFINITY;
+  float m[kMostParts / 256], l[kMostParts / 256], top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kParts / 256; ++i) {
+  for (int i = 0; i < kMostParts / 256; ++i) {
     const int w = tid + 256 * i;
     m[i] = -INFINITY;
     l[i] = 0.0f;
@@ -955,7 +972,7 @@ __global__ __launch_bounds__(256) void paged_join(AttnArgs a) {
   const float ref = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kParts / 256; ++i) {
+  for (int i = 0; i < kMostParts / 256; ++i) {
     const float k = __builtin_amdgcn_exp2f(m[i] - ref);
     weight[tid + 256 * i] = k;
     sum += l[i] * k;
@@ -1061,10 +1078,11 @@ bool dealt(int64_t capacity, int64_t window) {
 }
 
 template <class E>
-int launch(const AttnArgs& a, bool deal, hipStream_t st) {
+int launch(AttnArgs a, bool deal, hipStream_t st) {
   const int64_t items = (int64_t)a.B * a.Hk * a.rb;
   if (deal) {
-    paged_attn<E, true><<<kParts, 256, 0, st>>>(a);
+    a.most = E::kBlocks * kCUs;
+    paged_attn<E, true><<<a.most, 256, 0, st>>>(a);
     const int rows = a.group < kRows ? a.group : kRows;
     paged_join<<<dim3((unsigned)items, (unsigned)rows), 256, 0, st>>>(a);
   } else {
@@ -1091,36 +1109,30 @@ int launch16(const AttnArgs& a, bool deal, hipStream_t st) {
 
 using namespace si;
 
-extern "C" size_t si_paged_attn_workspace_bytes(int64_t Hq, int64_t Hk, int64_t D, int64_t capacity,
+extern "C" size_t si_paged_attn_workspace_bytes(int64_t Hq, int64_t heads, int64_t D, int64_t capacity,
                                                 int64_t window) {
-  if (Hk <= 0 || Hq % Hk != 0 || D <= 0 || D > 128 || D % 8 != 0 || !dealt(capacity, window)) return 0;
-  const int64_t group = Hq / Hk, rows = group < kRows ? group : kRows;
-  return (size_t)(2 * kParts * rows * (D + 2)) * sizeof(float);
+  if (heads <= 0 || Hq % heads != 0 || D <= 0 || D > 128 || D % 8 != 0 || !dealt(capacity, window)) return 0;
+  const int64_t group = Hq / heads, rows = group < kRows ? group : kRows;
+  return (size_t)(2 * kMostParts * rows * (D + 2)) * sizeof(float);
 }
 
-extern "C" int si_paged_attn(const void* q, int q_dtype, int64_t B, int64_t Hq, int64_t q_stride_b,
-                             int64_t q_stride_h, int64_t Hk, int64_t D, const int32_t* table,
+extern "C" int si_paged_attn(const si_page_pool* pool, const void* q, int q_dtype, int64_t B, int64_t Hq,
+                             int64_t q_stride_b, int64_t q_stride_h, const int32_t* table,
                              int64_t table_stride, int64_t table_width, const int32_t* lengths,
-                             int64_t window, float scale, int64_t pages, int64_t page_size,
-                             int precision, int dtype, int64_t group, void* const* pool, void* out,
-                             float* lse, void* workspace, size_t workspace_bytes, si_stream_t stream) {
+                             int64_t window, float scale, void* out, float* lse, void* workspace,
+                             size_t workspace_bytes, si_stream_t stream) {
   clear_error();
-  SI_CHECK_ARG(dtype_ok(q_dtype) && dtype_ok(dtype), "si_paged_attn: unsupported dtype");
-  SI_CHECK_ARG(precision >= SI_PREC_FP32 && precision <= SI_PREC_INT4,
-               "si_paged_attn: precision %d is not 0..3", precision);
-  SI_CHECK_ARG(B >= 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && Hq < 65536 && D > 0 && D <= 512 &&
-               B * Hq < ((int64_t)1 << 31), "si_paged_attn: bad shape");
-  SI_CHECK_ARG(pages > 0 && page_size > 0 && pages < ((int64_t)1 << 31) && page_size < ((int64_t)1 << 31) &&
-               pages <= (((int64_t)1 << 31) - 1) / Hk / page_size,
-               "si_paged_attn: pools hold fewer than 2^31 rows");
-  SI_CHECK_ARG(table_width >= 0 && table_width <= (((int64_t)1 << 31) - 1 - 2 * kTile) / page_size,
+  const int rc = check_pool("si_paged_attn", pool);
+  if (rc != SI_OK) return rc;
+  const si_page_pool& p = *pool;
+  SI_CHECK_ARG(dtype_ok(q_dtype), "si_paged_attn: unsupported dtype %d", q_dtype);
+  SI_CHECK_ARG(B >= 0 && Hq > 0 && Hq < 65536 && Hq % p.heads == 0 && B < ((int64_t)1 << 31) / Hq,
+               "si_paged_attn: bad shape");
+  SI_CHECK_ARG(table_width >= 0 && table_width <= (((int64_t)1 << 31) - 1 - 2 * kTile) / p.page_size,
                "si_paged_attn: page tables reach fewer than 2^31 positions");
   SI_CHECK_ARG(window >= 0 && window < ((int64_t)1 << 31), "si_paged_attn: bad window");
-  SI_CHECK_ARG(group > 0 && D % group == 0, "si_paged_attn: group must divide D");
   if (B == 0) return SI_OK;
-  SI_CHECK_ARG(q && (table || table_width == 0) && lengths && pool && pool[0] && pool[1] && out,
-               "si_paged_attn: NULL argument");
-  SI_CHECK_ARG(precision < SI_PREC_INT8 || (pool[2] && pool[3]), "si_paged_attn: NULL scales");
+  SI_CHECK_ARG(q && (table || table_width == 0) && lengths && out, "si_paged_attn: NULL argument");
   AttnArgs a = {};
   a.q = q;
   a.qs[0] = q_stride_b;
@@ -1129,38 +1141,37 @@ extern "C" int si_paged_attn(const void* q, int q_dtype, int64_t B, int64_t Hq, 
   a.table = table;
   a.ts = table_stride;
   a.lens = lengths;
-  a.capacity = table_width * page_size;
+  a.capacity = table_width * p.page_size;
   a.B = (int)B;
-  a.Hk = (int)Hk;
-  a.group = (int)(Hq / Hk);
+  a.Hk = (int)p.heads;
+  a.group = (int)(Hq / p.heads);
   a.rb = (int)ceil_div(a.group, kRows);
-  a.P = (int)page_size;
+  a.P = (int)p.page_size;
   a.window = (int)window;
-  a.D = (int)D;
-  a.g = (int)group;
-  a.pages = pages;
+  a.D = (int)p.D;
+  a.g = (int)p.group;
+  a.pages = p.pages;
   a.scale = scale * kLog2e;
-  uintptr_t bits = 0;
-  for (int j = 0; j < 4; ++j) {
-    a.pool[j] = pool[j];
-    bits |= reinterpret_cast<uintptr_t>(pool[j]);
-  }
-  a.sdt = dtype;
+  a.pool[0] = p.k;
+  a.pool[1] = p.v;
+  a.pool[2] = p.scale_k;
+  a.pool[3] = p.scale_v;
+  a.sdt = (int)p.dtype;
   a.out = out;
   a.lse = lse;
   a.part_rows = a.group < kRows ? a.group : kRows;
-  const int kind = precision == SI_PREC_FP32 ? (dtype == SI_DT_F32 ? kF32 : dtype == SI_DT_F16 ? kF16 : kBF16)
-                   : precision == SI_PREC_FP16 ? kF16 : precision == SI_PREC_INT8 ? kI8 : kI4;
+  const int kind = p.precision == SI_PREC_FP32 ? (p.dtype == SI_DT_F32 ? kF32 : p.dtype == SI_DT_F16 ? kF16 : kBF16)
+                   : p.precision == SI_PREC_FP16 ? kF16 : p.precision == SI_PREC_INT8 ? kI8 : kI4;
   hipStream_t st = as_stream(stream);
   // chunks of eight values of a row, in one int4 group
-  const bool tiles = D <= 128 && D % 8 == 0 && (bits & 15) == 0 && (kind != kI4 || group % 8 == 0);
+  const bool tiles = a.D <= 128 && a.D % 8 == 0 && (kind != kI4 || a.g % 8 == 0);
   if (!tiles) {
     paged_attn_any<<<(unsigned)(B * Hq), 256, 0, st>>>(a, kind);
     return check_launch("si_paged_attn/any");
   }
   const bool deal = dealt(a.capacity, window);
   if (deal) {
-    const size_t need = si_paged_attn_workspace_bytes(Hq, Hk, D, a.capacity, window);
+    const size_t need = si_paged_attn_workspace_bytes(Hq, p.heads, a.D, a.capacity, window);
     SI_CHECK_ARG(workspace && workspace_bytes >= need, "si_paged_attn: workspace of %zu bytes needed, got %zu",
                  need, workspace ? workspace_bytes : (size_t)0);
     SI_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "si_paged_attn: workspace not 16-byte aligned");
@@ -1171,8 +1182,8 @@ extern "C" int si_paged_attn(const void* q, int q_dtype, int64_t B, int64_t Hq, 
     if (kind == kBF16)
       return q_dtype == SI_DT_BF16 ? launch16<kBF16, 1, 1>(a, deal, st) : launch16<kBF16, 2, 1>(a, deal, st);
     if (kind == kI8) return launch16<kI8, 1, 1>(a, deal, st);
-    if (kind == kI4 && D / group <= 8)
-      return dtype == SI_DT_BF16 ? launch16<kI4, 1, 1>(a, deal, st) : launch16<kI4, 1, 2>(a, deal, st);
+    if (kind == kI4 && a.D / a.g <= 8)
+      return a.sdt == SI_DT_BF16 ? launch16<kI4, 1, 1>(a, deal, st) : launch16<kI4, 1, 2>(a, deal, st);
   }
   switch (kind) {
     case kF32: return launch32<kF32>(a, deal, st);

@@ -9,6 +9,7 @@
 //
 // Both kernels move every byte once and are bound by HBM, at few tokens by the
 // launch and one chain of loads.
+#include "si_pool_args.h"
 #include "si_pool_index.h"
 #include "si_rotate.h"
 #include "si_row_quant.h"
@@ -314,33 +315,27 @@ __global__ __launch_bounds__(256) void pool_read_any(PoolArgs a) {
   }
 }
 
-int check_pool(const char* what, int dtype, int64_t T, int64_t H, int64_t D, int64_t pages, int64_t P,
-               int precision, int64_t group, void* const* pool, const int64_t* slots) {
-  SI_CHECK_ARG(dtype_ok(dtype), "%s: unsupported dtype %d", what, dtype);
-  SI_CHECK_ARG(precision >= SI_PREC_FP32 && precision <= SI_PREC_INT4, "%s: precision %d is not 0..3",
-               what, precision);
-  SI_CHECK_ARG(T >= 0 && H > 0 && D > 0 && D <= 1024 && pages > 0 && P > 0, "%s: bad shape", what);
-  SI_CHECK_ARG(H < 65536 && pages < ((int64_t)1 << 31) && P < ((int64_t)1 << 31) &&
-               pages <= (((int64_t)1 << 31) - 1) / H / P, "%s: pools hold fewer than 2^31 rows", what);
-  SI_CHECK_ARG(T < ((int64_t)1 << 31) / H, "%s: too many rows for one call", what);
-  SI_CHECK_ARG(group > 0 && D % group == 0, "%s: group must divide D", what);
-  SI_CHECK_ARG(pool && pool[0] && pool[1] && slots, "%s: NULL argument", what);
-  SI_CHECK_ARG(precision < SI_PREC_INT8 || (pool[2] && pool[3]), "%s: NULL scales", what);
+int check_rows(const char* what, const si_page_pool* p, int64_t T, const int64_t* slots) {
+  const int rc = check_pool(what, p);
+  if (rc != SI_OK) return rc;
+  SI_CHECK_ARG(T >= 0 && T < ((int64_t)1 << 31) / p->heads, "%s: bad row count", what);
+  SI_CHECK_ARG(slots || T == 0, "%s: NULL slots", what);
   return SI_OK;
 }
 
-PoolArgs pool_args(int64_t T, int64_t H, int64_t D, int64_t pages, int64_t P, int precision,
-                   int64_t group, void* const* pool, const int64_t* slots) {
+PoolArgs pool_args(const si_page_pool& p, int64_t T, const int64_t* slots) {
   PoolArgs a = {};
   a.T = T;
-  a.H = (int)H;
-  a.D = (int)D;
-  a.pages = pages;
-  a.P = (int)P;
-  a.prec = precision;
-  a.g = (int)group;
+  a.H = (int)p.heads;
+  a.D = (int)p.D;
+  a.pages = p.pages;
+  a.P = (int)p.page_size;
+  a.prec = (int)p.precision;
+  a.g = (int)p.group;
+  a.sdt = (int)p.dtype;
   a.slots = slots;
-  for (int j = 0; j < 4; ++j) a.pool.p[4 * precision + j] = pool[j];
+  void* const t[4] = {p.k, p.v, p.scale_k, p.scale_v};
+  for (int j = 0; j < 4; ++j) a.pool.p[4 * a.prec + j] = t[j];
   return a;
 }
 
@@ -363,8 +358,7 @@ void launch_write(const PoolArgs& a, bool rotated, hipStream_t st) {
 template <int DT>
 int write_rows(PoolArgs& a, bool rotated, hipStream_t st) {
   constexpr int EPL = Chunk<DT>::EPL;
-  const bool whole = (a.ks[0] | a.ks[1] | a.vs[0] | a.vs[1] | a.D) % EPL == 0 && aligned16(a.k, a.v) &&
-                     aligned16(a.pool.p[4 * a.prec], a.pool.p[4 * a.prec + 1]);
+  const bool whole = (a.ks[0] | a.ks[1] | a.vs[0] | a.vs[1] | a.D) % EPL == 0 && aligned16(a.k, a.v);
   int lpr = 8;
   while (lpr * EPL < a.D) lpr *= 2;
   // int4 groups of a power of two of lanes, or the whole row
@@ -391,62 +385,57 @@ int write_rows(PoolArgs& a, bool rotated, hipStream_t st) {
 
 using namespace si;
 
-extern "C" int si_pool_write(const void* k, const void* v, int dtype, int64_t T, int64_t H, int64_t D,
+extern "C" int si_pool_write(const si_page_pool* pool, const void* k, const void* v, int64_t T,
                              int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
-                             int64_t v_stride_h, const int64_t* slots, int64_t pages, int64_t page_size,
-                             int precision, int64_t group, void* const* pool, int64_t pairs,
-                             int interleaved, const double* freq, double gain, const void* positions,
-                             int positions64, int64_t pos_stride, si_stream_t stream) {
+                             int64_t v_stride_h, const int64_t* slots, const si_rotation* rotation,
+                             const void* positions, int positions64, int64_t pos_stride,
+                             si_stream_t stream) {
   clear_error();
-  if (T == 0) return SI_OK;
-  const int rc = check_pool("si_pool_write", dtype, T, H, D, pages, page_size, precision, group, pool, slots);
+  const int rc = check_rows("si_pool_write", pool, T, slots);
   if (rc != SI_OK) return rc;
+  if (rotation != nullptr)
+    SI_CHECK_ARG(rotation->pairs > 0 && 2 * rotation->pairs <= pool->D && rotation->freq && (positions || T == 0),
+                 "si_pool_write: bad rotation");
+  if (T == 0) return SI_OK;
   SI_CHECK_ARG(k && v, "si_pool_write: NULL argument");
-  SI_CHECK_ARG(pairs >= 0 && 2 * pairs <= D && (pairs == 0 || (freq && positions)),
-               "si_pool_write: bad rotation");
-  PoolArgs a = pool_args(T, H, D, pages, page_size, precision, group, pool, slots);
+  PoolArgs a = pool_args(*pool, T, slots);
   a.k = reinterpret_cast<const char*>(k);
   a.v = reinterpret_cast<const char*>(v);
   a.ks[0] = k_stride_t;
   a.ks[1] = k_stride_h;
   a.vs[0] = v_stride_t;
   a.vs[1] = v_stride_h;
-  a.sdt = dtype;
-  a.rot = {freq, positions, positions64, (int)pairs, interleaved ? 1 : 0, gain, 1.0};
+  const bool rotated = rotation != nullptr;
+  if (rotated) a.rot = to_rotation(*rotation, positions, positions64, false);
   a.pos_stride = pos_stride;
   hipStream_t st = as_stream(stream);
-  const bool rotated = pairs > 0;
-  if (dtype == SI_DT_F32) return write_rows<SI_DT_F32>(a, rotated, st);
-  if (dtype == SI_DT_F16) return write_rows<SI_DT_F16>(a, rotated, st);
+  if (a.sdt == SI_DT_F32) return write_rows<SI_DT_F32>(a, rotated, st);
+  if (a.sdt == SI_DT_F16) return write_rows<SI_DT_F16>(a, rotated, st);
   return write_rows<SI_DT_BF16>(a, rotated, st);
 }
 
-extern "C" int si_pool_read(const int64_t* slots, int64_t T, int64_t H, int64_t D, int64_t pages,
-                            int64_t page_size, int precision, int dtype, int64_t group,
-                            void* const* pool, void* out_k, void* out_v, int out_dtype,
-                            si_stream_t stream) {
+extern "C" int si_pool_read(const si_page_pool* pool, const int64_t* slots, int64_t T, void* out_k,
+                            void* out_v, int out_dtype, si_stream_t stream) {
   clear_error();
-  if (T == 0) return SI_OK;
-  const int rc = check_pool("si_pool_read", dtype, T, H, D, pages, page_size, precision, group, pool, slots);
+  const int rc = check_rows("si_pool_read", pool, T, slots);
   if (rc != SI_OK) return rc;
   SI_CHECK_ARG(dtype_ok(out_dtype), "si_pool_read: unsupported output dtype %d", out_dtype);
+  if (T == 0) return SI_OK;
   SI_CHECK_ARG(out_k && out_v, "si_pool_read: NULL argument");
-  PoolArgs a = pool_args(T, H, D, pages, page_size, precision, group, pool, slots);
+  PoolArgs a = pool_args(*pool, T, slots);
   a.ko = reinterpret_cast<char*>(out_k);
   a.vo = reinterpret_cast<char*>(out_v);
-  a.sdt = dtype;
   a.odt = out_dtype;
   hipStream_t st = as_stream(stream);
-  const bool vec = D % 8 == 0 && (precision != SI_PREC_INT4 || group % 8 == 0) && aligned16(out_k, out_v) &&
-                   aligned16(pool[0], pool[1]);
+  const bool vec = a.D % 8 == 0 && (a.prec != SI_PREC_INT4 || a.g % 8 == 0) && aligned16(out_k, out_v);
   if (!vec) {
-    SI_CHECK_ARG(ceil_div(T * H * D, 256) < ((int64_t)1 << 31), "si_pool_read: too many rows for one call");
-    pool_read_any<<<(unsigned)ceil_div(T * H * D, 256), 256, 0, st>>>(a);
+    SI_CHECK_ARG(ceil_div(T * a.H * a.D, 256) < ((int64_t)1 << 31), "si_pool_read: too many rows for one call");
+    pool_read_any<<<(unsigned)ceil_div(T * a.H * a.D, 256), 256, 0, st>>>(a);
     return check_launch("si_pool_read/any");
   }
   int lsh = 0;
-  while ((8 << lsh) < D) ++lsh;
-  const unsigned grid = (unsigned)(ceil_div(T, 256 >> lsh) * H);
+  while ((8 << lsh) < a.D) ++lsh;
+  const unsigned grid = (unsigned)(ceil_div(T, 256 >> lsh) * a.H);
   if (out_dtype == SI_DT_F32) pool_read<SI_DT_F32><<<grid, 256, 0, st>>>(a, lsh);
   else if (out_dtype == SI_DT_F16) pool_read<SI_DT_F16><<<grid, 256, 0, st>>>(a, lsh);
   else pool_read<SI_DT_BF16><<<grid, 256, 0, st>>>(a, lsh);

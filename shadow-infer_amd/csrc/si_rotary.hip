@@ -157,17 +157,18 @@ void launch(const RotaryArgs& a, dim3 grid, size_t lds, hipStream_t st) {
 
 using namespace si;
 
-extern "C" int si_rotary(const si_rotary_rows* q, const si_rotary_rows* k, int dtype, int64_t B,
-                         int64_t S, int64_t D, int64_t pairs, int interleaved, const double* freq,
-                         double gain, int transpose, const void* positions, int positions64,
-                         int64_t pos_stride_b, int64_t pos_stride_s, si_stream_t stream) {
+extern "C" int si_rotary(const si_rotation* rotation, const si_rotary_rows* q, const si_rotary_rows* k,
+                         int dtype, int64_t B, int64_t S, int64_t D, int transpose,
+                         const void* positions, int positions64, int64_t pos_stride_b,
+                         int64_t pos_stride_s, si_stream_t stream) {
   clear_error();
   SI_CHECK_ARG(dtype_ok(dtype), "si_rotary: unsupported dtype %d", dtype);
   SI_CHECK_ARG(B >= 0 && S >= 0 && B < ((int64_t)1 << 31) && S < ((int64_t)1 << 31) &&
                B * S < ((int64_t)1 << 31), "si_rotary: bad batch");
+  SI_CHECK_ARG(rotation != nullptr && q != nullptr, "si_rotary: NULL argument");
+  const int64_t pairs = rotation->pairs;
   SI_CHECK_ARG(D > 0 && D <= 1024 && pairs > 0 && 2 * pairs <= D,
                "si_rotary: need 0 < 2 * pairs <= D <= 1024");
-  SI_CHECK_ARG(q != nullptr, "si_rotary: NULL argument");
   RotaryArgs a = {};
   const si_rotary_rows* in[2] = {q, k};
   uintptr_t bits = 0;
@@ -190,8 +191,8 @@ extern "C" int si_rotary(const si_rotary_rows* q, const si_rotary_rows* k, int d
   if (tokens == 0 || heads == 0) return SI_OK;
   for (int j = 0; j < 2; ++j)
     SI_CHECK_ARG(a.t[j].heads == 0 || (a.t[j].src && a.t[j].dst), "si_rotary: NULL argument");
-  SI_CHECK_ARG(freq && positions, "si_rotary: NULL argument");
-  a.rot = {freq, positions, positions64, (int)pairs, interleaved ? 1 : 0, gain, transpose ? -1.0 : 1.0};
+  SI_CHECK_ARG(rotation->freq && positions, "si_rotary: NULL argument");
+  a.rot = to_rotation(*rotation, positions, positions64, transpose);
   a.ps[0] = pos_stride_b;
   a.ps[1] = pos_stride_s;
   a.tokens = tokens;

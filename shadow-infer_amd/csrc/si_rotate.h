@@ -18,6 +18,10 @@ struct Rotation {
   double sign;
 };
 
+inline Rotation to_rotation(const si_rotation& r, const void* positions, int positions64, bool transpose) {
+  return {r.freq, positions, positions64, (int)r.pairs, r.interleaved ? 1 : 0, r.gain, transpose ? -1.0 : 1.0};
+}
+
 // cos and sin of t turns, times gain. The argument is reduced in 64 bits (the
 // integer part of t and then its nearest quarter are subtracted exactly), so
 // position 10^6 is as exact as position 1; |x| <= pi/4 is left, where the Taylor

@@ -35,7 +35,6 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _sz = ctypes.c_size_t
-_f64 = ctypes.c_double
 _PTR16 = ctypes.c_void_p * 16
 _PTR4 = ctypes.c_void_p * 4
 
@@ -121,16 +120,13 @@ _SIGNATURES = {
                                       _sz, _vp]),
     "si_int8_linear_forward_add": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
                                           _vp, _sz, _vp]),
-    "si_rotary": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i32, _vp, _f64, _i32, _vp, _i32,
-                         _i64, _i64, _vp]),
-    "si_pool_write": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64,
-                             _i64, _i32, _i64, _vp, _i64, _i32, _vp, _f64, _vp, _i32, _i64, _vp]),
-    "si_pool_read": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i64, _vp, _vp, _vp,
-                            _i32, _vp]),
+    "si_rotary": (_i32, [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32, _i64, _i64, _vp]),
+    "si_pool_write": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i64,
+                             _vp]),
+    "si_pool_read": (_i32, [_vp, _vp, _i64, _vp, _vp, _i32, _vp]),
     "si_paged_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
-    "si_paged_attn": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp,
-                             _i64, ctypes.c_float, _i64, _i64, _i32, _i32, _i64, _vp, _vp, _vp, _vp,
-                             _sz, _vp]),
+    "si_paged_attn": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+                             ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
     "si_int8_linear_forward_noalloc": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
                                               _vp]),
 }
@@ -201,14 +197,14 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name}: {msg} (status {rc})")
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with torch's current stream on ``device`` as the last argument. A
-    launch goes to the current device, so that is made ``device`` where it is not."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        call(name, *args, stream(device))
+def call_on(index: int, name: str, *args) -> None:
+    """``call`` with torch's current stream on device ``index`` as the last argument.
+    A launch goes to the current device, so that is made ``index`` where it is not."""
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
         return
-    with torch.cuda.device(device):
-        call(name, *args, stream(device))
+    with torch.cuda.device(index):
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def size_query(name: str, *args) -> int:

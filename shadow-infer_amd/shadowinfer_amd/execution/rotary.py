@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 from typing import List, Optional, Tuple, Union
 
@@ -118,37 +119,47 @@ class RotaryEmbedding:
         # turns per position, in fp64 on the device
         self.turns = torch.tensor([x / (2.0 * math.pi) for x in angles], dtype=torch.float64,
                                   device=self.device)
+        self._spec = ctypes.create_string_buffer(struct.pack(  # si_rotation
+            "=qqQd", size // 2, 1 if layout == "interleaved" else 0, self.turns.data_ptr(),
+            self.value_factor))
 
-    def _rows(self, x: torch.Tensor, what: str, inplace: bool):
-        if x.dim() not in (3, 4) or x.shape[-1] != self.head_dim:
-            raise ValueError(f"{what} must be [tokens, heads, {self.head_dim}] or "
-                             f"[batch, tokens, heads, {self.head_dim}], got {tuple(x.shape)}")
+    def _rows(self, x: torch.Tensor, shape, what: str, inplace: bool):
+        """(source, output, their si_rotary_rows). The source may be a copy."""
+        s = x.stride()
         if inplace:
-            if x.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
-                raise ValueError(f"{what} cannot be rotated in place: strides {x.stride()}")
-            out = x
+            if s[-1] != 1 or 0 in s and any(a == 0 and n > 1 for a, n in zip(s, shape)):
+                raise ValueError(f"{what} cannot be rotated in place: strides {s}")
+            out, o = x, s
         else:
-            if x.stride(-1) != 1:
+            if s[-1] != 1:
                 x = x.contiguous()
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        s, o = x.stride(), out.stride()
-        sb, ob = (s[0], o[0]) if x.dim() == 4 else (0, 0)
-        return x, out, _ROWS(x.data_ptr(), out.data_ptr(), x.shape[-2], sb, s[-3], s[-2], ob, o[-3],
-                             o[-2])
+                s = x.stride()
+            out = torch.empty_like(x)
+            o = out.stride()
+            if o[-1] != 1:  # of an expanded tensor
+                out = torch.empty_like(x, memory_format=torch.contiguous_format)
+                o = out.stride()
+        if len(s) == 4:
+            rows = _ROWS(x.data_ptr(), out.data_ptr(), shape[2], s[0], s[1], s[2], o[0], o[1], o[2])
+        else:
+            rows = _ROWS(x.data_ptr(), out.data_ptr(), shape[1], 0, s[0], s[1], 0, o[0], o[1])
+        return x, out, rows
 
-    def check_positions(self, positions: torch.Tensor, lead: torch.Size,
-                        device: torch.device) -> Tuple[int, int]:
-        """Refuses positions that are not one integer per token of ``lead``
-        (``[S]`` also serves every row of ``[B, S]``); returns their element
-        strides between batches and tokens."""
-        if positions.dtype not in (torch.int64, torch.int32):
+    def check_positions(self, positions: torch.Tensor, lead, index: int) -> Tuple[int, int, int]:
+        """Refuses positions that are not one integer per token of ``lead`` on
+        device ``index`` (``[S]`` also serves every row of ``[B, S]``); returns
+        whether they are int64 and their element strides between batches and
+        tokens."""
+        wide = positions.dtype is torch.int64
+        if not wide and positions.dtype is not torch.int32:
             raise TypeError(f"positions must be int64 or int32, got {positions.dtype}")
-        if positions.device != device:
-            raise ValueError(f"positions must be on {device}, got {positions.device}")
-        if positions.shape != lead and not (len(lead) == 2 and positions.shape == lead[1:]):
-            raise ValueError(f"positions must be {list(lead)}, got {list(positions.shape)}")
+        if positions.get_device() != index:
+            raise ValueError(f"positions must be on device {index}, got {positions.device}")
+        shape = positions.shape
+        if shape != lead and not (len(lead) == 2 and shape == lead[1:]):
+            raise ValueError(f"positions must be {list(lead)}, got {list(shape)}")
         s = positions.stride()
-        return (s[0] if len(s) == 2 else 0), s[-1]
+        return wide, (s[0] if len(s) == 2 else 0), s[-1]
 
     def __call__(self, positions: torch.Tensor, q: torch.Tensor, k: Optional[torch.Tensor] = None,
                  *, transpose: bool = False, inplace: bool = False
@@ -160,26 +171,31 @@ class RotaryEmbedding:
         other way: the gradient of this call with respect to its input, and,
         where ``value_factor`` is 1, its inverse. ``inplace=True`` writes into q
         and k. Not recorded by autograd."""
-        _native.require_device(q, "RotaryEmbedding")
-        if self.turns.device != q.device:
+        index = q.get_device()
+        if index < 0:
+            _native.require_device(q, "RotaryEmbedding")
+        if index != self.turns.get_device():
             raise ValueError(f"this RotaryEmbedding is on {self.turns.device}, q on {q.device}")
         code = _native.dtype_code(q.dtype)
-        lead = q.shape[:-2]
+        shape = q.shape
+        if len(shape) not in (3, 4) or shape[-1] != self.head_dim:
+            raise ValueError(f"q must be [tokens, heads, {self.head_dim}] or [batch, tokens, heads, "
+                             f"{self.head_dim}], got {tuple(shape)}")
+        lead = shape[:-2]
         if k is not None:
-            if k.dtype != q.dtype or k.device != q.device:
+            if k.dtype is not q.dtype or k.get_device() != index:
                 raise ValueError("q and k must share device and dtype")
-            if k.shape[:-2] != lead:
-                raise ValueError(f"q and k must hold the same tokens, got {tuple(q.shape)} and "
-                                 f"{tuple(k.shape)}")
+            kshape = k.shape
+            if len(kshape) != len(shape) or kshape[:-2] != lead or kshape[-1] != self.head_dim:
+                raise ValueError("q and k must hold the same tokens, got "
+                                 f"{tuple(shape)} and {tuple(kshape)}")
+        wide, pb, ps = self.check_positions(positions, lead, index)
         # sources stay bound until the launch is queued
-        src_q, out_q, rows_q = self._rows(q, "q", inplace)
-        src_k, out_k, rows_k = (None, None, None) if k is None else self._rows(k, "k", inplace)
-        pb, ps = self.check_positions(positions, lead, q.device)
-        B, S = (lead[0], lead[1]) if len(lead) == 2 else (1, lead[0])
-        _native.call_on(q.device, "si_rotary", rows_q, rows_k, code, B, S, self.head_dim,
-                        self.rotary_dim // 2, 1 if self.layout == "interleaved" else 0,
-                        self.turns.data_ptr(), self.value_factor, 1 if transpose else 0,
-                        positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0, pb, ps)
+        src_q, out_q, rows_q = self._rows(q, shape, "q", inplace)
+        src_k, out_k, rows_k = (None, None, None) if k is None else self._rows(k, kshape, "k", inplace)
+        B, S = lead if len(lead) == 2 else (1, lead[0])
+        _native.call_on(index, "si_rotary", self._spec, rows_q, rows_k, code, B, S, self.head_dim,
+                        transpose, positions.data_ptr(), wide, pb, ps)
         return out_q if k is None else (out_q, out_k)
 
     def __repr__(self) -> str:

@@ -11,6 +11,7 @@ calls capture into graphs.
 
 from __future__ import annotations
 
+import ctypes
 from typing import Any, Optional, Tuple
 
 import torch
@@ -18,6 +19,7 @@ import torch
 from .. import _native
 
 _PREC_CODE = {"fp32": 0, "fp16": 1, "int8": 2, "int4": 3}
+_SPEC = ctypes.c_int64 * 11  # si_page_pool
 
 
 class KVPagePool:
@@ -62,7 +64,10 @@ class KVPagePool:
         self._k, self._v = zeros(row, payload), zeros(row, payload)
         self._sk = None if scales is None else zeros(scales, dtype)
         self._sv = None if scales is None else zeros(scales, dtype)
-        self._table = _native.table4([_native.ptr(t) for t in (self._k, self._v, self._sk, self._sv)])
+        self._spec = _SPEC(self.num_pages, self.num_heads, self.page_size, self.head_dim,
+                           _PREC_CODE[precision], self._dtype_code, self.int4_group_size,
+                           *(_native.ptr(t) or 0 for t in (self._k, self._v, self._sk, self._sv)))
+        self._index = self._k.get_device()
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
@@ -78,13 +83,16 @@ class KVPagePool:
         return sum(t.numel() * t.element_size() for t in (self._k, self._v, self._sk, self._sv)
                    if t is not None)
 
-    def _check_slots(self, slots: torch.Tensor) -> None:
-        if slots.dtype != torch.int64:
+    def _rows(self, slots: torch.Tensor) -> int:
+        """The number of slots; refuses what is not an int64 vector on the pool's device."""
+        if slots.dtype is not torch.int64:
             raise TypeError(f"slots must be int64, got {slots.dtype}")
-        if slots.dim() != 1:
-            raise ValueError(f"slots must be [tokens], got {tuple(slots.shape)}")
-        if slots.device != self._k.device:
+        if slots.get_device() != self._index:
             raise ValueError(f"slots must be on the pool's device ({self._k.device}), got {slots.device}")
+        shape = slots.shape
+        if len(shape) != 1:
+            raise ValueError(f"slots must be [tokens], got {tuple(shape)}")
+        return shape[0]
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, rotary=None,
               positions: Optional[torch.Tensor] = None) -> None:
@@ -95,54 +103,59 @@ class KVPagePool:
         be open. With ``rotary`` (a RotaryEmbedding) K is rotated to
         ``positions`` ``[T]`` on its way, to the bytes that rotating first would
         give."""
-        _native.require_device(k, "KVPagePool.write")
-        if k.dim() != 3 or k.shape[1:] != (self.num_heads, self.head_dim) or v.shape != k.shape:
-            raise ValueError(f"k and v must be [tokens, {self.num_heads}, {self.head_dim}], got "
-                             f"{tuple(k.shape)} and {tuple(v.shape)}")
-        if k.dtype != self.dtype or v.dtype != self.dtype:
+        index = self._index
+        if k.get_device() < 0 or index < 0:
+            _native.require_device(k, "KVPagePool.write")
+            _native.require_device(self._k, "KVPagePool.write")
+        if k.dtype is not self.dtype or v.dtype is not self.dtype:
             raise TypeError(f"k and v must be {self.dtype}, got {k.dtype} and {v.dtype}")
-        if k.device != self._k.device or v.device != self._k.device:
+        if k.get_device() != index or v.get_device() != index:
             raise ValueError(f"k and v must be on the pool's device ({self._k.device})")
-        self._check_slots(slots)
-        T = k.shape[0]
-        if slots.shape[0] != T:
-            raise ValueError(f"need {T} slots, got {slots.shape[0]}")
-        turn = (0, 0, None, 1.0, None, 0, 0)
+        shape = k.shape
+        if len(shape) != 3 or shape[1] != self.num_heads or shape[2] != self.head_dim or v.shape != shape:
+            raise ValueError(f"k and v must be [tokens, {self.num_heads}, {self.head_dim}], got "
+                             f"{tuple(shape)} and {tuple(v.shape)}")
+        T = self._rows(slots)
+        if T != shape[0]:
+            raise ValueError(f"need {shape[0]} slots, got {T}")
+        spec, at, wide, step = None, None, 0, 0
         if rotary is not None:
             if positions is None:
                 raise ValueError("rotary needs positions")
-            if rotary.head_dim != self.head_dim or rotary.turns.device != k.device:
+            if rotary.head_dim != self.head_dim or rotary.turns.get_device() != index:
                 raise ValueError("rotary must have the pool's head_dim and device")
-            _, step = rotary.check_positions(positions, k.shape[:1], k.device)
-            turn = (rotary.rotary_dim // 2, 1 if rotary.layout == "interleaved" else 0,
-                    rotary.turns.data_ptr(), rotary.value_factor, positions.data_ptr(),
-                    1 if positions.dtype == torch.int64 else 0, step)
+            wide, _, step = rotary.check_positions(positions, shape[:1], index)
+            spec, at = rotary._spec, positions.data_ptr()
         elif positions is not None:
             raise ValueError("positions are of use with rotary only")
         # copies stay bound until the launch is queued
-        kc = k if k.stride(2) == 1 else k.contiguous()
-        vc = v if v.stride(2) == 1 else v.contiguous()
-        sc = slots.contiguous()
-        _native.call_on(k.device, "si_pool_write", kc.data_ptr(), vc.data_ptr(), self._dtype_code, T,
-                        self.num_heads, self.head_dim, kc.stride(0), kc.stride(1), vc.stride(0),
-                        vc.stride(1), sc.data_ptr(), self.num_pages, self.page_size,
-                        _PREC_CODE[self.precision], self.int4_group_size, self._table, *turn)
+        ks, vs = k.stride(), v.stride()
+        if ks[2] != 1:
+            k = k.contiguous()
+            ks = k.stride()
+        if vs[2] != 1:
+            v = v.contiguous()
+            vs = v.stride()
+        if T > 1 and slots.stride(0) != 1:
+            slots = slots.contiguous()
+        _native.call_on(index, "si_pool_write", self._spec, k.data_ptr(), v.data_ptr(), T, ks[0], ks[1],
+                        vs[0], vs[1], slots.data_ptr(), spec, at, wide, step)
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float32
              ) -> Tuple[torch.Tensor, torch.Tensor]:
         """(k, v) ``[T, heads, head_dim]`` of the slots (int64 ``[T]``) in
         ``dtype``: the values the stored rows stand for, zeros for a slot outside
         the pool."""
-        _native.require_device(self._k, "KVPagePool.read")
-        self._check_slots(slots)
-        T = slots.shape[0]
+        if self._index < 0:
+            _native.require_device(self._k, "KVPagePool.read")
+        T = self._rows(slots)
         code = _native.dtype_code(dtype)
-        sc = slots.contiguous()
-        k = torch.empty(T, self.num_heads, self.head_dim, dtype=dtype, device=self._k.device)
+        if T > 1 and slots.stride(0) != 1:
+            slots = slots.contiguous()
+        k = torch.empty((T, self.num_heads, self.head_dim), dtype=dtype, device=self._k.device)
         v = torch.empty_like(k)
-        _native.call_on(k.device, "si_pool_read", sc.data_ptr(), T, self.num_heads, self.head_dim,
-                        self.num_pages, self.page_size, _PREC_CODE[self.precision], self._dtype_code,
-                        self.int4_group_size, self._table, k.data_ptr(), v.data_ptr(), code)
+        _native.call_on(self._index, "si_pool_read", self._spec, slots.data_ptr(), T, k.data_ptr(),
+                        v.data_ptr(), code)
         return k, v
 
     def __repr__(self) -> str:

@@ -13,7 +13,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from .. import _native
-from .page_pool import _PREC_CODE, KVPagePool
+from .page_pool import KVPagePool
 
 
 def paged_attention(q: torch.Tensor, pool: KVPagePool, page_table: torch.Tensor,
@@ -31,38 +31,46 @@ def paged_attention(q: torch.Tensor, pool: KVPagePool, page_table: torch.Tensor,
     pool (-1: dropped) take no part, lengths are cut to the table, negative ones
     are 0. A sequence without positions gives zeros and -inf. Several query heads
     of one kv head share its read; scores, softmax and sums are fp32."""
-    _native.require_device(q, "paged_attention")
-    if q.dim() != 3 or q.shape[2] != pool.head_dim or q.shape[1] == 0 or q.shape[1] % pool.num_heads:
+    index = q.get_device()
+    if index < 0:
+        _native.require_device(q, "paged_attention")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != pool.head_dim or shape[1] == 0 or shape[1] % pool.num_heads:
         raise ValueError(f"q must be [sequences, heads, {pool.head_dim}] with heads a multiple of "
-                         f"{pool.num_heads}, got {tuple(q.shape)}")
+                         f"{pool.num_heads}, got {tuple(shape)}")
     code = _native.dtype_code(q.dtype)
-    B, H, D = q.shape
-    dev = q.device
-    if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+    B, H, D = shape
+    if page_table.dtype is not torch.int32 or lengths.dtype is not torch.int32:
         raise TypeError(f"page_table and lengths must be int32, got {page_table.dtype} and "
                         f"{lengths.dtype}")
-    if page_table.dim() != 2 or page_table.shape[0] != B or lengths.shape != (B,):
+    tshape = page_table.shape
+    if len(tshape) != 2 or tshape[0] != B or lengths.shape != shape[:1]:
         raise ValueError(f"need a page table [{B}, pages] and lengths [{B}], got "
-                         f"{tuple(page_table.shape)} and {tuple(lengths.shape)}")
-    if pool.k.device != dev or page_table.device != dev or lengths.device != dev:
+                         f"{tuple(tshape)} and {tuple(lengths.shape)}")
+    if pool._index != index or page_table.get_device() != index or lengths.get_device() != index:
         raise ValueError("q, the pool, page_table and lengths must be on one device")
-    if window is not None and not 1 <= window < 1 << 31:
+    if window is None:
+        window = 0
+    elif not 1 <= window < 1 << 31:
         raise ValueError(f"window must be >= 1 (and below 2**31), got {window}")
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
     # copies stay bound until the launch is queued
-    qc = q if q.stride(2) == 1 else q.contiguous()
-    table = page_table if page_table.shape[1] < 2 or page_table.stride(1) == 1 else page_table.contiguous()
-    lens = lengths.contiguous()
-    out = torch.empty(B, H, D, dtype=q.dtype, device=dev)
-    lse = torch.empty(B, H, dtype=torch.float32, device=dev) if return_lse else None
-    width = page_table.shape[1]
+    qs, ts, width = q.stride(), page_table.stride(), tshape[1]
+    if qs[2] != 1:
+        q = q.contiguous()
+        qs = q.stride()
+    if ts[1] != 1 and width > 1:
+        page_table = page_table.contiguous()
+        ts = page_table.stride()
+    if B > 1 and lengths.stride(0) != 1:
+        lengths = lengths.contiguous()
+    out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     ws_bytes = _native.size_query("si_paged_attn_workspace_bytes", H, pool.num_heads, D,
-                                  width * pool.page_size, window or 0)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    _native.call_on(dev, "si_paged_attn", qc.data_ptr(), code, B, H, qc.stride(0), qc.stride(1),
-                    pool.num_heads, D, table.data_ptr(), table.stride(0), width, lens.data_ptr(),
-                    window or 0, float(sm_scale), pool.num_pages, pool.page_size,
-                    _PREC_CODE[pool.precision], pool._dtype_code, pool.int4_group_size, pool._table,
+                                  width * pool.page_size, window)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    _native.call_on(index, "si_paged_attn", pool._spec, q.data_ptr(), code, B, H, qs[0], qs[1],
+                    page_table.data_ptr(), ts[0], width, lengths.data_ptr(), window, float(sm_scale),
                     out.data_ptr(), _native.ptr(lse), _native.ptr(ws), ws_bytes)
     return (out, lse) if return_lse else out

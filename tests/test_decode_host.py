@@ -4,6 +4,7 @@ natively), rotary scalings, refusals, and known answers of the oracle."""
 import ctypes
 import math
 import os
+import struct
 import subprocess
 
 import numpy as np
@@ -120,43 +121,50 @@ def test_abi_refuses_before_any_launch():
     lib = _native.load()
     rows = (ctypes.c_int64 * 9)(16, 16, 2, 0, 128, 64, 0, 128, 64)
 
-    def rotary(dtype=2, B=1, S=4, D=64, pairs=32, q=rows, freq=16, pos=16):
-        return lib.si_rotary(q, None, dtype, B, S, D, pairs, 0, freq, 1.0, 0, pos, 1, 0, 1, None)
+    def rotation(pairs=32, freq=16):
+        return ctypes.create_string_buffer(struct.pack("=qqQd", pairs, 0, freq, 1.0))
+
+    def rotary(dtype=2, B=1, S=4, D=64, pairs=32, q=rows, freq=16, pos=16, spec=True):
+        return lib.si_rotary(rotation(pairs, freq) if spec else None, q, None, dtype, B, S, D, 0, pos, 1, 0,
+                             1, None)
 
     for kw in (dict(dtype=5), dict(D=0), dict(D=2048), dict(pairs=33), dict(pairs=0), dict(B=-1),
-               dict(S=1 << 31), dict(q=None), dict(freq=None), dict(pos=None)):
+               dict(S=1 << 31), dict(q=None), dict(freq=0), dict(pos=None), dict(spec=False)):
         assert rotary(**kw) == 1 and b"si_rotary" in lib.si_last_error(), kw
     assert rotary(S=0) == 0  # nothing to do
-    table = _native.table4([16, 16, 16, 16])
-    none = _native.table4([16, 16, None, None])
 
-    def write(dtype=2, T=4, H=2, D=64, pages=8, P=4, prec=2, g=16, pool=table, slots=16, pairs=0, freq=16):
-        return lib.si_pool_write(16, 16, dtype, T, H, D, 128, 64, 128, 64, slots, pages, P, prec, g,
-                                 pool, pairs, 0, freq, 1.0, 16, 1, 1, None)
+    def pool(pages=8, H=2, P=4, D=64, prec=2, dtype=2, g=16, k=16, v=16, sk=16, sv=16):
+        return (ctypes.c_int64 * 11)(pages, H, P, D, prec, dtype, g, k, v, sk, sv)
 
-    for kw in (dict(dtype=3), dict(prec=4), dict(prec=-1), dict(T=-1), dict(H=0), dict(D=0), dict(D=1025),
-               dict(pages=0), dict(P=0), dict(pages=1 << 30, P=4), dict(pages=1 << 40), dict(g=24),
-               dict(pool=None), dict(pool=none), dict(slots=None), dict(pairs=33), dict(pairs=-1),
-               dict(pairs=8, freq=None), dict(T=1 << 31)):
+    bad = [dict(pages=0), dict(pages=1 << 40), dict(pages=1 << 30, P=4), dict(H=0), dict(H=65536), dict(P=0),
+           dict(D=0), dict(D=513, g=1), dict(prec=4), dict(prec=-1), dict(dtype=3), dict(dtype=1 << 32),
+           dict(g=24), dict(g=0), dict(k=0), dict(v=0), dict(sk=0), dict(sv=0), dict(k=8), dict(sv=24)]
+    specs = [pool(**kw) for kw in bad] + [None]
+
+    def write(spec=pool(), T=4, k=16, slots=16, turn=None, pos=16):
+        return lib.si_pool_write(spec, k, 16, T, 128, 64, 128, 64, slots, turn, pos, 1, 1, None)
+
+    def read(spec=pool(), T=4, slots=16, out=16, odt=0):
+        return lib.si_pool_read(spec, slots, T, out, 16, odt, None)
+
+    def attn(spec=pool(P=128), qdt=2, B=2, Hq=4, width=4, win=0, q=16, table=16, lens=16, out=16, ws=16,
+             size=1 << 30):
+        return lib.si_paged_attn(spec, q, qdt, B, Hq, 256, 64, table, 4, width, lens, win, 0.125, out, None, ws,
+                                 size, None)
+
+    for f, name in ((write, b"si_pool_write"), (read, b"si_pool_read"), (attn, b"si_paged_attn")):
+        for spec in specs:
+            assert f(spec=spec) == 1 and name in lib.si_last_error(), (name, spec and list(spec))
+    for kw in (dict(T=-1), dict(T=1 << 31), dict(slots=None), dict(k=None), dict(turn=rotation(33)),
+               dict(turn=rotation(0)), dict(turn=rotation(8, 0)), dict(turn=rotation(8), pos=None)):
         assert write(**kw) == 1 and b"si_pool_write" in lib.si_last_error(), kw
     assert write(T=0) == 0
-
-    def read(T=4, prec=2, pool=table, out=16, odt=0, g=16):
-        return lib.si_pool_read(16, T, 2, 64, 8, 4, prec, 2, g, pool, out, 16, odt, None)
-
-    for kw in (dict(prec=7), dict(pool=none), dict(out=None), dict(odt=4), dict(g=0), dict(T=1 << 31)):
+    for kw in (dict(T=-1), dict(T=1 << 31), dict(slots=None), dict(out=None), dict(odt=4)):
         assert read(**kw) == 1 and b"si_pool_read" in lib.si_last_error(), kw
     assert read(T=0) == 0
-
-    def attn(qdt=2, B=2, Hq=4, Hk=2, D=64, width=4, win=0, pages=8, P=128, prec=2, dtype=2, g=16,
-             pool=table, q=16, lens=16, ws=16, size=1 << 30):
-        return lib.si_paged_attn(q, qdt, B, Hq, 256, 64, Hk, D, 16, 4, width, lens, win,
-                                 0.125, pages, P, prec, dtype, g, pool, 16, None, ws, size, None)
-
-    for kw in (dict(qdt=3), dict(dtype=9), dict(prec=4), dict(Hq=3), dict(Hk=0), dict(D=0), dict(D=513),
-               dict(B=-1), dict(pages=0), dict(pages=1 << 30), dict(width=-1), dict(width=1 << 25),
-               dict(win=-1), dict(win=1 << 31), dict(g=24), dict(pool=none), dict(pool=None), dict(q=None),
-               dict(lens=None), dict(ws=None), dict(size=8)):
+    for kw in (dict(qdt=3), dict(Hq=3), dict(Hq=0), dict(B=-1), dict(B=1 << 30), dict(width=-1),
+               dict(width=1 << 25), dict(win=-1), dict(win=1 << 31), dict(q=None), dict(table=None),
+               dict(lens=None), dict(out=None), dict(ws=None), dict(ws=24), dict(size=8)):
         assert attn(**kw) == 1 and b"si_paged_attn" in lib.si_last_error(), kw
     assert attn(B=0) == 0
     size = lib.si_paged_attn_workspace_bytes
