@@ -671,11 +671,11 @@ int si_pool_read(const si_page_pool* pool, const int64_t* slots, int64_t T, void
  * [B, Hq, D] in q's dtype, lse [B, Hq] (natural logarithm; or NULL). No position:
  * out 0, lse -inf. The workspace (device, 16-byte aligned; capacity = table_width *
  * page_size) may be 0 bytes where the size query says so. */
-size_t si_paged_attn_workspace_bytes(int64_t Hq, int64_t heads, int64_t D, int64_t capacity,
-                                     int64_t window);
+size_t si_paged_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t heads, int64_t D,
+                                     int64_t capacity, int64_t window);
 int si_paged_attn(const si_page_pool* pool, const void* q, int q_dtype, int64_t B, int64_t Hq,
                   int64_t q_stride_b, int64_t q_stride_h, const int32_t* table, int64_t table_stride,
-                  int64_t table_width, const int32_t* lengths, int64_t window, float scale, void* out,
+                  int64_t table_width, const int32_t* lengths, int64_t window, double scale, void* out,
                   float* lse, void* workspace, size_t workspace_bytes, si_stream_t stream);
 
 #ifdef __cplusplus

@@ -124,9 +124,9 @@ _SIGNATURES = {
     "si_pool_write": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i64,
                              _vp]),
     "si_pool_read": (_i32, [_vp, _vp, _i64, _vp, _vp, _i32, _vp]),
-    "si_paged_attn_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "si_paged_attn_workspace_bytes": (_sz, [_i64] * 6),
     "si_paged_attn": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
-                             ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
+                             ctypes.c_double, _vp, _vp, _vp, _sz, _vp]),
     "si_int8_linear_forward_noalloc": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
                                               _vp]),
 }
@@ -191,20 +191,26 @@ def call(name: str, *args) -> None:
     lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
-        msg = lib.si_last_error().decode(errors="replace")
-        if rc == 1:
-            raise ValueError(f"{name}: {msg}")
-        raise RuntimeError(f"{name}: {msg} (status {rc})")
+        _failed(name, rc)
+
+
+def _failed(name: str, rc: int) -> None:
+    msg = _lib.si_last_error().decode(errors="replace")
+    if rc == 1:
+        raise ValueError(f"{name}: {msg}")
+    raise RuntimeError(f"{name}: {msg} (status {rc})")
 
 
 def call_on(index: int, name: str, *args) -> None:
     """``call`` with torch's current stream on device ``index`` as the last argument.
     A launch goes to the current device, so that is made ``index`` where it is not."""
-    if index == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-        return
-    with torch.cuda.device(index):
-        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return call_on(index, name, *args)
+    _refuse_forced_cpu(name)
+    rc = getattr(_lib or load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _failed(name, rc)
 
 
 def size_query(name: str, *args) -> int:

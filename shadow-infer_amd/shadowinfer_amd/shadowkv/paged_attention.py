@@ -67,7 +67,7 @@ def paged_attention(q: torch.Tensor, pool: KVPagePool, page_table: torch.Tensor,
         lengths = lengths.contiguous()
     out = torch.empty(shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    ws_bytes = _native.size_query("si_paged_attn_workspace_bytes", H, pool.num_heads, D,
+    ws_bytes = _native.size_query("si_paged_attn_workspace_bytes", B, H, pool.num_heads, D,
                                   width * pool.page_size, window)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     _native.call_on(index, "si_paged_attn", pool._spec, q.data_ptr(), code, B, H, qs[0], qs[1],

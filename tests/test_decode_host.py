@@ -147,7 +147,7 @@ def test_abi_refuses_before_any_launch():
     def read(spec=pool(), T=4, slots=16, out=16, odt=0):
         return lib.si_pool_read(spec, slots, T, out, 16, odt, None)
 
-    def attn(spec=pool(P=128), qdt=2, B=2, Hq=4, width=4, win=0, q=16, table=16, lens=16, out=16, ws=16,
+    def attn(spec=pool(P=128), qdt=2, B=2, Hq=4, width=8, win=0, q=16, table=16, lens=16, out=16, ws=16,
              size=1 << 30):
         return lib.si_paged_attn(spec, q, qdt, B, Hq, 256, 64, table, 4, width, lens, win, 0.125, out, None, ws,
                                  size, None)
@@ -168,8 +168,9 @@ def test_abi_refuses_before_any_launch():
         assert attn(**kw) == 1 and b"si_paged_attn" in lib.si_last_error(), kw
     assert attn(B=0) == 0
     size = lib.si_paged_attn_workspace_bytes
-    assert size(4, 2, 64, 512, 0) > 0 and size(4, 2, 64, 512, 0) == size(4, 2, 64, 1 << 20, 0)
-    assert size(4, 3, 64, 512, 0) == 0 and size(4, 0, 64, 512, 0) == 0
+    assert size(1, 4, 2, 64, 4096, 0) > 0 and size(1, 4, 2, 64, 4096, 0) == size(9, 4, 2, 64, 1 << 20, 0)
+    assert size(1, 4, 2, 64, 4096, 100) == 0 and size(1, 4, 2, 64, 100, 0) == 0
+    assert size(1, 4, 3, 64, 4096, 0) == 0 and size(1, 4, 0, 64, 4096, 0) == 0
 
 
 # ------------------------------------------------------------------- oracle
