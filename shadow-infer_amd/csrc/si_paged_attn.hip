@@ -41,6 +41,7 @@ struct AttnArgs {
   int64_t capacity;         // positions of a table row
   int B, Hk, group, rb;     // rb: row blocks of a group
   int P, window, D, g;
+  si_divisor by_page;       // divides by P
   int64_t pages;
   float scale, scale_lo;    // times log2(e), and what fp32 leaves of that
   const void* pool[4];      // k, v, scale_k, scale_v
@@ -67,6 +68,11 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
   return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// Memory that no kernel writes while this one runs, read through scalar loads.
+__device__ __forceinline__ const __attribute__((address_space(4))) int32_t* scalar(const int32_t* p) {
+  return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
 }
 
 // v, computed again where it is used: what is derived from it is not kept in
@@ -202,8 +208,10 @@ __device__ __forceinline__ void widen(const uint32_t* w, float* x) {
   }
 }
 
-// EXACT: D == DP, and wider loads of K.
-template <int KIND, int DP_, bool EXACT, bool FP32, int NQ, int NS>
+// EXACT: D == DP, and wider loads of K. EIGHTS: eight positions from a multiple of
+// eight on lie in one page, so a tile's rows are four runs whose first ones are
+// scalars; otherwise each lane finds one position's row and they go through LDS.
+template <int KIND, int DP_, bool EXACT, bool EIGHTS, bool FP32, int NQ, int NS>
 struct Engine {
   static constexpr int DP = DP_, J = DP / 16, M = DP / 32;
   // Blocks of a CU, for the registers' bound and the dealing.
@@ -218,18 +226,22 @@ struct Engine {
   static constexpr int kVW1 = kVW ? kVW : 1;
   static constexpr int kUnit = 8 * kBits / 32;  // words of eight values
 
-  // A wave's LDS: rows [32], then per position: K's factor, V's factor, its logarithm,
-  // and int4's scales as [32][kG] for K and [kG][32] for V, s' in NS fp16 parts each or
+  // A wave's LDS: rows [32], then per position K's factor and V's factor, and int4's
+  // scales as [32][kG] for K and [kG][32] for V, s' in NS fp16 parts each or
   // fp32.
   static constexpr int kLdsScale = 32 * 4;
-  static constexpr int kLdsParts = kLdsScale + (kScaled ? 3 * 32 * 4 : 0);
+  static constexpr int kLdsParts = kLdsScale + (kScaled ? 2 * 32 * 4 : 0);
   static constexpr int kLds = kLdsParts + (KIND == kI4 ? 2 * 32 * kG * (FP32 ? 4 : 2 * NS) : 0);
 
   uint32_t k[2][kKW], v[2][4][kVW1];  // a tile's rows
   uint32_t sc[KIND == kI4 ? (FP32 ? 16 : NS == 1 ? 4 : 8) : 1];
-  int32_t row;    // of position lane % 32
+  uint32_t next_live;
+  int32_t row;    // of position lane % 32 (-1: takes no part)
   uint32_t live;  // bit 4 s + i: position s * 16 + 4 kq + i takes part
-  int32_t t0, end, page;  // the wave's position, where its tiles end, the next one's table entry
+  int32_t t0, end;  // the wave's position, and where its tiles end
+  // The next tile's table entries: of position lane % 32, or of the four eights. Then
+  // the first rows of the eights that are being loaded.
+  int32_t page[EIGHTS ? 4 : 1], run[EIGHTS ? 4 : 1];
 
   Running<J> st;
   u4 q[NQ][M];
@@ -293,26 +305,91 @@ struct Engine {
     }
   }
 
-  // The page table entry of position t + lane % 32.
-  __device__ __forceinline__ static int32_t entry(const AttnArgs& a, int b, int32_t t, int32_t hi) {
-    t += threadIdx.x & 31;
-    return t < hi ? a.table[b * a.ts + (uint32_t)t / (uint32_t)a.P] : -1;
+  // The page table entries of the tile at t.
+  __device__ __forceinline__ void find_pages(const AttnArgs& a, int b, int32_t t, int32_t hi) {
+    if constexpr (EIGHTS) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        page[g] = t + 8 * g < hi ? scalar(a.table)[b * a.ts + si_divide(t + 8 * g, a.by_page)] : -1;
+    } else {
+      t += threadIdx.x & 31;
+      page[0] = t < hi ? a.table[b * a.ts + si_divide(t, a.by_page)] : -1;
+    }
   }
 
-  // Starts the loads of the keys and scales of the tile at t0, its rows into LDS.
-  // Positions that do not take part read row 0.
-  __device__ __forceinline__ void start_keys(const AttnArgs& a, int32_t* lds_rows, int hk, int32_t hi) {
-    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
+  // The tile's rows, from its table entries.
+  __device__ __forceinline__ void find_rows(const AttnArgs& a, int32_t* lds_rows, int hk, int32_t lo, int32_t hi) {
+    const int lane = threadIdx.x & 63, kq = lane >> 4;
     const int32_t t = t0 + (lane & 31);
-    row = t < hi ? si_page_row(page, a.pages, hk, a.Hk, (int32_t)((uint32_t)t % (uint32_t)a.P), a.P) : -1;
-    if (lane < 32) lds_rows[lane] = row;
-    wave_sync();
+    if constexpr (EIGHTS) {
+      bool all = t0 >= lo && t0 + kWaveTokens <= hi;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int32_t u = t0 + 8 * g;
+        run[g] = si_page_row(page[g], a.pages, hk, a.Hk, u - (int32_t)si_divide(u, a.by_page) * a.P, a.P);
+        all = all && run[g] >= 0;
+      }
+      if constexpr (kScaled) {
+        // (copies: a choice between members would put them all into memory)
+        int32_t r[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) r[g] = afresh(run[g]);
+        const int32_t lower = lane & 8 ? r[1] : r[0], upper = lane & 8 ? r[3] : r[2], first = lane & 16 ? upper : lower;
+        row = first >= 0 && t >= lo && t < hi ? first + (lane & 7) : -1;
+      }
+      next_live = 0xffu;
+      if (!all) {
+        next_live = 0;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int32_t u = t0 + s * 16 + kq * 4 + i;
+            const bool there = kq & 2 ? run[2 * s + 1] >= 0 : run[2 * s] >= 0;
+            if (there && u >= lo && u < hi) next_live |= 1u << (4 * s + i);
+          }
+        }
+      }
+    } else {
+      row = t >= lo && t < hi
+                ? si_page_row(page[0], a.pages, hk, a.Hk, t - (int32_t)si_divide(t, a.by_page) * a.P, a.P) : -1;
+      if (lane < 32) lds_rows[lane] = row;
+      wave_sync();
+      next_live = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int4 r4 = *reinterpret_cast<const int4*>(lds_rows + s * 16 + kq * 4);
+        const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r[i] >= 0) next_live |= 1u << (4 * s + i);
+      }
+    }
+  }
+
+  static constexpr int kRowBytes = EXACT ? DP * kBits / 8 : 0;
+  __device__ __forceinline__ static int64_t row_bytes(const AttnArgs& a) {
+    return EXACT ? (int64_t)kRowBytes : (int64_t)a.D * kBits / 8;
+  }
+  // Bytes of run g from a tensor's start, for rows of n bytes; row 0 where there is none.
+  __device__ __forceinline__ int64_t run_at(int g, int64_t n) const { return (int64_t)(run[g] < 0 ? 0 : run[g]) * n; }
+
+  // Starts the loads of the keys and scales of the tile at t0. Positions that do not
+  // take part read row 0, or one of the eight rows from their run's first on.
+  __device__ __forceinline__ void start_keys(const AttnArgs& a, int32_t* lds_rows, int hk, int32_t lo, int32_t hi) {
+    const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
+    find_rows(a, lds_rows, hk, lo, hi);
     const char* kp = reinterpret_cast<const char*>(a.pool[0]);
-    const int64_t row_bytes = (int64_t)a.D * kBits / 8;
+    const int64_t n = row_bytes(a);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int32_t r = lds_rows[s * 16 + c];
-      const char* p = kp + (r < 0 ? 0 : r) * row_bytes;
+      const char* p;
+      if constexpr (EIGHTS) {
+        p = (c < 8 ? kp + run_at(2 * s, n) : kp + run_at(2 * s + 1, n)) + (c & 7) * (int)n;
+      } else {
+        const int32_t r = lds_rows[s * 16 + c];
+        p = kp + (r < 0 ? 0 : r) * n;
+      }
       if constexpr (EXACT) {
         // 16 bytes a load: 64 bytes of a row by its four lanes
         if constexpr (kBits >= 16) {
@@ -352,8 +429,8 @@ struct Engine {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               const uint16_t* h = reinterpret_cast<const uint16_t*>(sp) + r * G + 2 * w;
-              const uint32_t lo = 2 * w < G ? h[0] : 0, hi16 = 2 * w + 1 < G ? h[1] : 0;
-              sc[w] = lo | (hi16 << 16);
+              const uint32_t lo16 = 2 * w < G ? h[0] : 0, hi16 = 2 * w + 1 < G ? h[1] : 0;
+              sc[w] = lo16 | (hi16 << 16);
             }
           }
         } else {
@@ -364,23 +441,30 @@ struct Engine {
     }
   }
 
-  // Starts the loads of its values; which of the lane's positions take part.
+  // Starts the loads of its values.
   __device__ __forceinline__ void start_values(const AttnArgs& a, const int32_t* lds_rows) {
     const int lane = threadIdx.x & 63, c = lane & 15, kq = lane >> 4;
     const char* vp = reinterpret_cast<const char*>(a.pool[1]);
-    const int64_t row_bytes = (int64_t)a.D * kBits / 8;
-    live = 0;
+    const int64_t n = row_bytes(a);
+    live = next_live;
     const bool in = EXACT || c * J < a.D;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int4 r4 = *reinterpret_cast<const int4*>(lds_rows + s * 16 + kq * 4);
-      const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
+      const char* p[4];
+      if constexpr (EIGHTS) {
+        p[0] = (kq & 2 ? vp + run_at(2 * s + 1, n) : vp + run_at(2 * s, n)) + (kq & 1) * 4 * (int)n + c * J * kBits / 8;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) p[i] = p[0] + i * n;
+      } else {
+        const int4 r4 = *reinterpret_cast<const int4*>(lds_rows + s * 16 + kq * 4);
+        const int32_t r[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = vp + (r[i] < 0 ? 0 : r[i]) * n + c * J * kBits / 8;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (r[i] >= 0) live |= 1u << (4 * s + i);
-        const char* p = vp + (r[i] < 0 ? 0 : r[i]) * row_bytes + c * J * kBits / 8;
         if (in) {
-          load_words<kVW>(p, v[s][i]);
+          load_words<kVW>(p[i], v[s][i]);
         } else {
 #pragma unroll
           for (int w = 0; w < kVW1; ++w) v[s][i][w] = KIND == kI4 ? 0x88888888u : 0u;
@@ -389,10 +473,24 @@ struct Engine {
     }
   }
 
+  // The factors of the lane's own positions s * 16 + 4 kq + i (j: 0 K, 1 V): an int8 row's
+  // scale, 2^e of an int4 row's, 0 for a position that takes no part.
+  __device__ __forceinline__ static f32x4 factors(const char* lds, int j, int s) {
+    const int kq = (threadIdx.x & 63) >> 4;
+    return *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + kLdsScale) + 32 * j + s * 16 + kq * 4);
+  }
+
+  // At least log2 of a factor: 1 + the mantissa is at most 0.0861 below 2^mantissa. (A
+  // factor below 2^-80 or not a number: its weight needs no more room than this.)
+  __device__ __forceinline__ static float log2_bound(float f) {
+    const float x = fmaxf(__builtin_fmaf((float)(int)__float_as_uint(f), 0x1p-23f, -126.913f), -80.0f);
+    return f < INFINITY ? x : -80.0f;
+  }
+
   // The tile's scales into the wave's LDS.
   __device__ __forceinline__ void place_scales(const AttnArgs& a, char* lds) const {
     const int lane = threadIdx.x & 63, t = lane & 31;
-    float* factor = reinterpret_cast<float*>(lds + kLdsScale);  // [3][32]
+    float* factor = reinterpret_cast<float*>(lds + kLdsScale);  // [2][32]
     float f = 1.0f;
     if constexpr (KIND == kI8) {
       f = a.sdt == SI_DT_F32 ? __uint_as_float(sc[0])
@@ -430,13 +528,7 @@ struct Engine {
         }
       }
     }
-    if (lane < 32) {
-      factor[t] = f;
-    } else {
-      factor[32 + t] = f;
-      // (a scale below 2^-80 or not a number: its weight needs no more room than this)
-      if constexpr (!FP32) factor[64 + t] = fminf(fmaxf(__builtin_amdgcn_logf(f), -80.0f), 127.0f);
-    }
+    factor[lane] = f;
     wave_sync();
   }
 
@@ -529,14 +621,16 @@ struct Engine {
 
   // Its weights and their products with the values.
   __device__ __forceinline__ void values(const AttnArgs& a, const char* lds, const f32x4* acc) {
-    const int kq = (threadIdx.x & 63) >> 4;
-    const float* factor = reinterpret_cast<const float*>(lds + kLdsScale);
     float w[8], y[8], top = st.m;
+    f32x4 vf[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      f32x4 kf = {1.0f, 1.0f, 1.0f, 1.0f}, lg = {0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (kScaled) kf = *reinterpret_cast<const f32x4*>(factor + s * 16 + kq * 4);
-      if constexpr (kScaled && !FP32) lg = *reinterpret_cast<const f32x4*>(factor + 64 + s * 16 + kq * 4);
+      f32x4 kf = {1.0f, 1.0f, 1.0f, 1.0f};
+      vf[s] = kf;
+      if constexpr (kScaled) {
+        kf = factors(lds, 0, s);
+        vf[s] = factors(lds, 1, s);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float x = acc[s][i];
@@ -549,7 +643,7 @@ struct Engine {
         }
         if (!(live >> (4 * s + i) & 1)) x = -INFINITY;
         y[4 * s + i] = x;
-        top = fmaxf(top, x + lg[i]);
+        top = fmaxf(top, kScaled && !FP32 ? x + log2_bound(vf[s][i]) : x);
       }
     }
     top = max_over_kq(top);
@@ -563,13 +657,11 @@ struct Engine {
     const float ref = st.m == -INFINITY ? 0.0f : st.m - kRoom;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      f32x4 vf = {1.0f, 1.0f, 1.0f, 1.0f};
-      if constexpr (kScaled) vf = *reinterpret_cast<const f32x4*>(factor + 32 + s * 16 + kq * 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float e = __builtin_amdgcn_exp2f(y[4 * s + i] - ref);
         st.l += e;
-        w[4 * s + i] = kScaled ? e * vf[i] : e;
+        w[4 * s + i] = kScaled ? e * vf[s][i] : e;
       }
     }
     if constexpr (FP32) products32(a, lds, w);
@@ -671,31 +763,33 @@ struct Engine {
     st.l = 0.0f;
 #pragma unroll
     for (int j = 0; j < J; ++j) st.o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    t0 = lo + ta * kTile + (threadIdx.x >> 6) * kWaveTokens;
-    end = tb * (int64_t)kTile + lo < hi ? lo + tb * kTile : hi;
+    const int32_t from = si_span_origin(lo);
+    t0 = from + ta * kTile + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kWaveTokens;
+    end = tb * (int64_t)kTile + from < hi ? from + tb * kTile : hi;
     if (t0 >= end) return;
     int32_t* rows = reinterpret_cast<int32_t*>(lds);
-    page = entry(a, b, t0, hi);
-    start_keys(a, rows, hk, hi);
+    find_pages(a, b, t0, hi);
+    start_keys(a, rows, hk, lo, hi);
     start_values(a, rows);
-    page = entry(a, b, t0 + kTile, hi);
+    find_pages(a, b, t0 + kTile, hi);
   }
 
   // All its tiles. A tile's keys are loaded over the last one's once its scores are
   // done, its values once its products are.
-  __device__ __forceinline__ void walk(const AttnArgs& a, char* lds, int b, int hk, int32_t hi) {
+  __device__ __forceinline__ void walk(const AttnArgs& a, char* lds, int b, int hk, int32_t lo, int32_t hi) {
     if (t0 >= end) return;
     int32_t* rows = reinterpret_cast<int32_t*>(lds);
     f32x4 acc[2];
     while (true) {
       scores(a, lds, acc);
       t0 += kTile;
-      if (t0 < end) {
-        start_keys(a, rows, hk, hi);
-        page = entry(a, b, t0 + kTile, hi);
+      const bool more = t0 < end;
+      if (more) {
+        start_keys(a, rows, hk, lo, hi);
+        find_pages(a, b, t0 + kTile, hi);
       }
       values(a, lds, acc);
-      if (t0 >= end) break;
+      if (!more) break;
       start_values(a, rows);
     }
     st.m -= kRoom;  // the sums are of weights scaled by 2^kRoom
@@ -783,7 +877,7 @@ __global__ __launch_bounds__(256, E::kBlocks) void paged_attn(AttnArgs a) {
     }
     __syncthreads();
     e.begin(a, lds_o[0]);
-    e.walk(a, mine, b, hk, hi);
+    e.walk(a, mine, b, hk, lo, hi);
 
     // the four waves' results together
     const int t1 = afresh(tid), lane = t1 & 63, wave = t1 >> 6, c = lane & 15, kq = lane >> 4;
@@ -1021,12 +1115,18 @@ int launch(AttnArgs a, bool deal, hipStream_t st) {
   return check_launch("si_paged_attn");
 }
 
-template <int KIND, bool FP32, int NQ, int NS>
+template <int KIND, bool EIGHTS, bool FP32, int NQ, int NS>
 int launch_size(const AttnArgs& a, bool deal, hipStream_t st) {
-  if (a.D == 64) return launch<Engine<KIND, 64, true, FP32, NQ, NS>>(a, deal, st);
-  if (a.D == 128) return launch<Engine<KIND, 128, true, FP32, NQ, NS>>(a, deal, st);
-  return a.D < 64 ? launch<Engine<KIND, 64, false, FP32, NQ, NS>>(a, deal, st)
-                  : launch<Engine<KIND, 128, false, FP32, NQ, NS>>(a, deal, st);
+  if (a.D == 64) return launch<Engine<KIND, 64, true, EIGHTS, FP32, NQ, NS>>(a, deal, st);
+  if (a.D == 128) return launch<Engine<KIND, 128, true, EIGHTS, FP32, NQ, NS>>(a, deal, st);
+  return a.D < 64 ? launch<Engine<KIND, 64, false, EIGHTS, FP32, NQ, NS>>(a, deal, st)
+                  : launch<Engine<KIND, 128, false, EIGHTS, FP32, NQ, NS>>(a, deal, st);
+}
+
+template <int KIND, bool FP32, int NQ, int NS>
+int launch_pages(const AttnArgs& a, bool deal, hipStream_t st) {
+  return a.P % 8 == 0 ? launch_size<KIND, true, FP32, NQ, NS>(a, deal, st)
+                      : launch_size<KIND, false, FP32, NQ, NS>(a, deal, st);
 }
 
 }  // namespace
@@ -1073,6 +1173,7 @@ extern "C" int si_paged_attn(const si_page_pool* pool, const void* q, int q_dtyp
   a.group = (int)(Hq / p.heads);
   a.rb = (int)ceil_div(a.group, kRows);
   a.P = (int)p.page_size;
+  a.by_page = si_make_divisor((uint32_t)p.page_size);
   a.window = (int)window;
   a.D = (int)p.D;
   a.g = (int)p.group;
@@ -1105,20 +1206,20 @@ extern "C" int si_paged_attn(const si_page_pool* pool, const void* q, int q_dtyp
     a.parts = reinterpret_cast<float*>(workspace);
   }
   if (q_dtype != SI_DT_F32) {
-    if (kind == kF16) return launch_size<kF16, false, 1, 1>(a, deal, st);
+    if (kind == kF16) return launch_pages<kF16, false, 1, 1>(a, deal, st);
     if (kind == kBF16)
-      return q_dtype == SI_DT_BF16 ? launch_size<kBF16, false, 1, 1>(a, deal, st)
-                                   : launch_size<kBF16, false, 2, 1>(a, deal, st);
-    if (kind == kI8) return launch_size<kI8, false, 1, 1>(a, deal, st);
+      return q_dtype == SI_DT_BF16 ? launch_pages<kBF16, false, 1, 1>(a, deal, st)
+                                   : launch_pages<kBF16, false, 2, 1>(a, deal, st);
+    if (kind == kI8) return launch_pages<kI8, false, 1, 1>(a, deal, st);
     if (kind == kI4 && a.D / a.g <= 8)
-      return a.sdt == SI_DT_BF16 ? launch_size<kI4, false, 1, 1>(a, deal, st)
-                                 : launch_size<kI4, false, 1, 2>(a, deal, st);
+      return a.sdt == SI_DT_BF16 ? launch_pages<kI4, false, 1, 1>(a, deal, st)
+                                 : launch_pages<kI4, false, 1, 2>(a, deal, st);
   }
   switch (kind) {
-    case kF32: return launch_size<kF32, true, 1, 1>(a, deal, st);
-    case kF16: return launch_size<kF16, true, 1, 1>(a, deal, st);
-    case kBF16: return launch_size<kBF16, true, 1, 1>(a, deal, st);
-    case kI8: return launch_size<kI8, true, 1, 1>(a, deal, st);
-    default: return launch_size<kI4, true, 1, 1>(a, deal, st);
+    case kF32: return launch_pages<kF32, true, 1, 1>(a, deal, st);
+    case kF16: return launch_pages<kF16, true, 1, 1>(a, deal, st);
+    case kBF16: return launch_pages<kBF16, true, 1, 1>(a, deal, st);
+    case kI8: return launch_pages<kI8, true, 1, 1>(a, deal, st);
+    default: return launch_pages<kI4, true, 1, 1>(a, deal, st);
   }
 }

@@ -36,8 +36,26 @@ SI_HD int32_t si_span_hi(int32_t length, int64_t capacity) {
 SI_HD int32_t si_span_lo(int32_t hi, int32_t window) {
   return window > 0 && hi > window ? hi - window : 0;
 }
+// Tiles start at a multiple of eight, so that eight positions from there lie in one
+// page where the page size is one too; the positions before lo are masked.
+SI_HD int32_t si_span_origin(int32_t lo) { return lo & ~7; }
 SI_HD int32_t si_span_tiles(int32_t lo, int32_t hi, int32_t tile) {
-  return (int32_t)(((int64_t)hi - lo + tile - 1) / tile);
+  return hi > lo ? (int32_t)(((int64_t)hi - si_span_origin(lo) + tile - 1) / tile) : 0;
+}
+
+// t / d for 0 <= t < 2^31 by a multiplication (the round-up method: with 2^shift the
+// power of two from d on, m = floor(2^32 (2^shift - d) / d) + 1).
+typedef struct {
+  uint32_t m, shift;
+} si_divisor;
+static inline si_divisor si_make_divisor(uint32_t d) {
+  si_divisor r = {0, 0};
+  while (((uint64_t)1 << r.shift) < d) ++r.shift;
+  r.m = (uint32_t)(((((uint64_t)1 << r.shift) - d) << 32) / d + 1);
+  return r;
+}
+SI_HD uint32_t si_divide(uint32_t t, si_divisor d) {
+  return ((uint32_t)(((uint64_t)t * d.m) >> 32) + t) >> d.shift;
 }
 
 // Workgroups that share `total` tiles: each has one at least.

@@ -4,7 +4,8 @@
  *
  *  1. rows of slots and of table entries are in [0, pages * heads * page_size) or -1,
  *     distinct slots have distinct rows, and pages or slots outside give -1;
- *  2. spans: [lo, hi) within [0, capacity], at most `window` long, tiles cover it;
+ *  2. spans: [lo, hi) within [0, capacity], at most `window` long, tiles cover it from a
+ *     multiple of eight; divisions by a multiplication are exact below 2^31;
  *  3. dealing, walked as the kernel walks it: every tile of every item is taken once,
  *     every block has at least one tile, an item that one block takes whole leaves no
  *     partial, no partial slot is written twice or past 2 * most, and the join of an
@@ -58,9 +59,23 @@ static void spans(void) {
   CHECK(lo >= 0 && lo <= hi && hi <= cap && (len < 0 ? hi == 0 : hi <= len));
   CHECK(hi == (len < 0 ? 0 : len < cap ? len : cap));
   CHECK(win ? hi - lo == (hi < win ? hi : win) : lo == 0);
-  CHECK((int64_t)n * 128 >= hi - lo && (int64_t)(n - 1) * 128 < (hi - lo > 0 ? hi - lo : 1));
+  const int32_t from = si_span_origin(lo);
+  CHECK(from % 8 == 0 && from <= lo && from > lo - 8 && (hi == lo) == (n == 0));
+  if (n) CHECK(from + (int64_t)n * 128 >= hi && from + (int64_t)(n - 1) * 128 < hi);
   const int32_t big = si_span_hi(2147483647, 2147483647LL - 128);
   CHECK(si_span_tiles(0, big, 128) == 16777215 && big == 2147483519);
+}
+
+static void divisions(void) {
+  const uint32_t d = rnd(40) ? (uint32_t)(1 + rnd(5000)) : (uint32_t)(1 + rnd(2147483647));
+  const si_divisor v = si_make_divisor(d);
+  for (int i = 0; i < 200; ++i) {
+    uint32_t t = (uint32_t)rnd(2147483648u);
+    if (i % 4 == 1) t = (uint32_t)(t / d * d);                    /* a multiple */
+    if (i % 4 == 2) t = t >= d ? t / d * d - 1 : 0;              /* just below one */
+    if (i == 3) t = 2147483647u;
+    CHECK(si_divide(t, v) == t / d);
+  }
 }
 
 static void dealing(int most) {
@@ -133,6 +148,7 @@ int main(void) {
   large_rows();
   for (int i = 0; i < 2000; ++i, ++cases) rows();
   for (int i = 0; i < 20000; ++i, ++cases) spans();
+  for (int i = 0; i < 20000; ++i, ++cases) divisions();
   const int most[4] = {1, 7, 64, 512};
   for (int i = 0; i < 800; ++i, ++cases) dealing(most[i % 4]);
   printf("cases %ld\n", cases);
