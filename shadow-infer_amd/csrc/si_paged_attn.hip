@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kRows = 16;        // query heads of an item
 constexpr int kWaveTokens = 32;
-constexpr int kTile = 4 * kWaveTokens;
+constexpr int kTile = 4 * kWaveTokens;  // of a dealt launch
 constexpr int kCUs = 256;
 constexpr int kMostParts = 4 * kCUs;  // workgroups of a dealt launch at most
 constexpr double kLog2e = 1.4426950408889634;
@@ -57,10 +57,10 @@ struct AttnArgs {
 enum { kF32 = 0, kF16 = 1, kBF16 = 2, kI8 = 3, kI4 = 4 };
 
 // Tiles of sequence b's items, and the first of its positions.
-__device__ __forceinline__ int span_tiles(const AttnArgs& a, int b, int32_t* lo, int32_t* hi) {
+__device__ __forceinline__ int span_tiles(const AttnArgs& a, int b, int32_t* lo, int32_t* hi, int tile = kTile) {
   *hi = si_span_hi(a.lens[b], a.capacity);
   *lo = si_span_lo(*hi, a.window);
-  return si_span_tiles(*lo, *hi, kTile);
+  return si_span_tiles(*lo, *hi, tile);
 }
 
 // A value that is the same in every lane, in scalar registers.
@@ -213,6 +213,7 @@ __device__ __forceinline__ void widen(const uint32_t* w, float* x) {
 // scalars; otherwise each lane finds one position's row and they go through LDS.
 template <int KIND, int DP_, bool EXACT, bool EIGHTS, bool FP32, int NQ, int NS>
 struct Engine {
+  static constexpr int kKind = KIND;
   static constexpr int DP = DP_, J = DP / 16, M = DP / 32;
   // Blocks of a CU, for the registers' bound and the dealing.
   static constexpr int kBlocks = KIND == kF32 ? 1 : KIND == kI8 || (KIND == kI4 && !FP32) ? 3 : 2;
@@ -756,7 +757,8 @@ struct Engine {
     }
   }
 
-  // The loads of the wave's first tile of [ta, tb).
+  // The loads of the wave's first tile of the block's [ta, tb), tiles of STEP positions.
+  template <int STEP>
   __device__ __forceinline__ void start(const AttnArgs& a, char* lds, int b, int hk, int32_t lo, int32_t hi,
                                         int32_t ta, int32_t tb) {
     st.m = -INFINITY;
@@ -764,29 +766,30 @@ struct Engine {
 #pragma unroll
     for (int j = 0; j < J; ++j) st.o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const int32_t from = si_span_origin(lo);
-    t0 = from + ta * kTile + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kWaveTokens;
-    end = tb * (int64_t)kTile + from < hi ? from + tb * kTile : hi;
+    t0 = from + ta * STEP + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kWaveTokens;
+    end = tb * (int64_t)STEP + from < hi ? from + tb * STEP : hi;
     if (t0 >= end) return;
     int32_t* rows = reinterpret_cast<int32_t*>(lds);
     find_pages(a, b, t0, hi);
     start_keys(a, rows, hk, lo, hi);
     start_values(a, rows);
-    find_pages(a, b, t0 + kTile, hi);
+    find_pages(a, b, t0 + STEP, hi);
   }
 
   // All its tiles. A tile's keys are loaded over the last one's once its scores are
   // done, its values once its products are.
+  template <int STEP>
   __device__ __forceinline__ void walk(const AttnArgs& a, char* lds, int b, int hk, int32_t lo, int32_t hi) {
     if (t0 >= end) return;
     int32_t* rows = reinterpret_cast<int32_t*>(lds);
     f32x4 acc[2];
     while (true) {
       scores(a, lds, acc);
-      t0 += kTile;
+      t0 += STEP;
       const bool more = t0 < end;
       if (more) {
         start_keys(a, rows, hk, lo, hi);
-        find_pages(a, b, t0 + kTile, hi);
+        find_pages(a, b, t0 + STEP, hi);
       }
       values(a, lds, acc);
       if (!more) break;
@@ -801,16 +804,18 @@ __device__ __forceinline__ float* part_sums(const AttnArgs& a) {
   return a.parts + (int64_t)2 * a.most * a.part_rows * a.D;
 }
 
-// DEALT: tiles dealt evenly to a.most blocks, partial results in a.parts. Otherwise
-// block = item, which it finishes.
-template <class E, bool DEALT>
-__global__ __launch_bounds__(256, E::kBlocks) void paged_attn(AttnArgs a) {
-  constexpr int DP = E::DP, J = DP / 16;
+// DEALT: tiles dealt evenly to a.most blocks of four waves, partial results in a.parts.
+// Otherwise block = item, which its W waves finish.
+template <class E, bool DEALT, int W>
+__global__ __launch_bounds__(64 * W, W == 4 ? E::kBlocks : 1) void paged_attn(AttnArgs a) {
+  static_assert(W == 4 || (W == 8 && !DEALT), "four waves, or eight over a whole item");
+  constexpr int DP = E::DP, kThreads = 64 * W, QN = kRows * DP / kThreads, kStep = W * kWaveTokens;
+  constexpr int J = DP / 16;
   // the waves' outputs; before, the query rows (in the first) and the waves' own memory
   constexpr int kOut = kRows * (DP + 4) * (int)sizeof(float);
-  __shared__ __attribute__((aligned(16))) char lds[kOut + (3 * kOut > 4 * E::kLds ? 3 * kOut : 4 * E::kLds)];
+  __shared__ __attribute__((aligned(16))) char lds[kOut + ((W - 1) * kOut > W * E::kLds ? (W - 1) * kOut : W * E::kLds)];
   float (*lds_o)[kRows][DP + 4] = reinterpret_cast<float (*)[kRows][DP + 4]>(lds);
-  __shared__ float lds_m[4][kRows], lds_l[4][kRows];
+  __shared__ float lds_m[W][kRows], lds_l[W][kRows];
   __shared__ int64_t lds_scan[8];
   const int tid = threadIdx.x;
   const int per = a.Hk * a.rb;  // items of a sequence
@@ -854,32 +859,32 @@ __global__ __launch_bounds__(256, E::kBlocks) void paged_attn(AttnArgs a) {
   }
 
   while (true) {
-    const int n = span_tiles(a, b, &lo, &hi);
+    const int n = span_tiles(a, b, &lo, &hi, kStep);
     const int32_t tb = !DEALT ? n : (int32_t)(ta + (end - f) < n ? ta + (end - f) : n);
     const int hk = item / a.rb, rb = item - hk * a.rb;
     const int rows = a.group - rb * kRows < kRows ? a.group - rb * kRows : kRows;
     const int64_t head0 = (int64_t)hk * a.group + rb * kRows;
 
     // the item's query rows in fp32 with zeros behind them, and the first rows' loads
-    float q[J];
+    float q[QN];
     const int t0 = afresh(tid);
 #pragma unroll
-    for (int i = 0; i < J; ++i) {
-      const int x = t0 + 256 * i, r = x / DP, d = x - r * DP;
+    for (int i = 0; i < QN; ++i) {
+      const int x = t0 + kThreads * i, r = x / DP, d = x - r * DP;
       q[i] = r < rows && d < a.D ? load_any(a.q, a.qdt, b * a.qs[0] + (head0 + r) * a.qs[1] + d) : 0.0f;
     }
     E e;
-    e.start(a, mine, b, hk, lo, hi, ta, tb);
+    e.template start<kStep>(a, mine, b, hk, lo, hi, ta, tb);
 #pragma unroll
-    for (int i = 0; i < J; ++i) {
-      const int x = t0 + 256 * i;
+    for (int i = 0; i < QN; ++i) {
+      const int x = t0 + kThreads * i;
       lds_o[0][x / DP][x % DP] = q[i];
     }
     __syncthreads();
     e.begin(a, lds_o[0]);
-    e.walk(a, mine, b, hk, lo, hi);
+    e.template walk<kStep>(a, mine, b, hk, lo, hi);
 
-    // the four waves' results together
+    // the waves' results together
     const int t1 = afresh(tid), lane = t1 & 63, wave = t1 >> 6, c = lane & 15, kq = lane >> 4;
     Running<J>& st = e.st;
     st.l += __shfl_xor(st.l, 16, 64);
@@ -898,13 +903,15 @@ __global__ __launch_bounds__(256, E::kBlocks) void paged_attn(AttnArgs a) {
     __syncthreads();
     const bool whole = ta == 0 && tb == n;
     const int64_t slot = DEALT ? si_part_slot(blockIdx.x, ta > 0) : 0;
-    for (int x = t1; x < rows * DP; x += 256) {
+    for (int x = t1; x < rows * DP; x += kThreads) {
       const int r = x / DP, d = x - r * DP;
       float top = -INFINITY;
-      for (int w = 0; w < 4; ++w) top = fmaxf(top, lds_m[w][r]);
+#pragma unroll
+      for (int w = 0; w < W; ++w) top = fmaxf(top, lds_m[w][r]);
       const float ref = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f, val = 0.0f;
-      for (int w = 0; w < 4; ++w) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
         const float k = __builtin_amdgcn_exp2f(lds_m[w][r] - ref);
         sum += lds_l[w][r] * k;
         val += lds_o[w][r][d] * k;
@@ -1091,14 +1098,16 @@ __global__ __launch_bounds__(256) void paged_attn_any(AttnArgs a, int kind) {
   if (tid == 0 && a.lse) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-// Whether an item's tiles are dealt (and joined), by the most it can have. Measured
-// with 32 query and 8 kv heads over int8 rows, whole items against dealt ones:
-// 2 tiles of 1 / 64 sequences 8.2 / 11.6 against 13.3 / 27 us, 4 tiles 11.7 / 16.2
-// against 13.3 / 28.7, 7 tiles 17.8 / 24 against 13.4 / 37, 13 tiles 29 / 51 against
-// 13.7 / 57, 25 tiles 52 / 92 against 14.9 / 87.
+// Whether items' tiles are dealt (and joined), by the most tiles one can have: whole
+// items take about 2 us for 256 positions (eight waves), dealt ones a second launch and
+// its chain. Measured with 32 query and 8 kv heads over int8 rows, whole against dealt,
+// us: 1 sequence (8 items) of 600 positions 10.5 / 13.4, 800 12.5 / 13.3, 1000 14.4 /
+// 13.3; 8 of 1000 15.9 / 16.7, 1600 21.1 / 19.2; 24 of 1600 22.3 / 29.9, 2400 30.1 / 33.4;
+// 64 of 2400 64.7 / 64.8.
 bool dealt(int64_t items, int64_t capacity, int64_t window) {
   const int64_t most = window > 0 && window < capacity ? window : capacity;
-  return most > (items >= 2 * kCUs ? 16 : 4) * kTile;
+  const int64_t limit = 6 + items / 16;
+  return most > (limit < 24 ? limit : 24) * kTile;
 }
 
 template <class E>
@@ -1106,11 +1115,15 @@ int launch(AttnArgs a, bool deal, hipStream_t st) {
   const int64_t items = (int64_t)a.B * a.Hk * a.rb;
   if (deal) {
     a.most = E::kBlocks * kCUs;
-    paged_attn<E, true><<<a.most, 256, 0, st>>>(a);
+    paged_attn<E, true, 4><<<a.most, 256, 0, st>>>(a);
     const int rows = a.group < kRows ? a.group : kRows;
     paged_join<<<dim3((unsigned)items, (unsigned)rows), 256, 0, st>>>(a);
+  } else if (items <= kCUs) {
+    // eight waves where a CU has one item at most: 1000 positions of 24 x 8 items 16.9
+    // us for 21.1 with four, of 64 x 8 items 34.2 for 30.1
+    paged_attn<E, false, 8><<<(unsigned)items, 512, 0, st>>>(a);
   } else {
-    paged_attn<E, false><<<(unsigned)items, 256, 0, st>>>(a);
+    paged_attn<E, false, 4><<<(unsigned)items, 256, 0, st>>>(a);
   }
   return check_launch("si_paged_attn");
 }

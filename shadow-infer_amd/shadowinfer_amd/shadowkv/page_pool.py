@@ -152,7 +152,7 @@ class KVPagePool:
         code = _native.dtype_code(dtype)
         if T > 1 and slots.stride(0) != 1:
             slots = slots.contiguous()
-        k = torch.empty((T, self.num_heads, self.head_dim), dtype=dtype, device=self._k.device)
+        k = self._k.new_empty((T, self.num_heads, self.head_dim), dtype=dtype)
         v = torch.empty_like(k)
         _native.call_on(self._index, "si_pool_read", self._spec, slots.data_ptr(), T, k.data_ptr(),
                         v.data_ptr(), code)

@@ -65,11 +65,11 @@ def paged_attention(q: torch.Tensor, pool: KVPagePool, page_table: torch.Tensor,
         ts = page_table.stride()
     if B > 1 and lengths.stride(0) != 1:
         lengths = lengths.contiguous()
-    out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    out = q.new_empty(shape)
+    lse = q.new_empty(shape[:2], dtype=torch.float32) if return_lse else None
     ws_bytes = _native.size_query("si_paged_attn_workspace_bytes", B, H, pool.num_heads, D,
                                   width * pool.page_size, window)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     _native.call_on(index, "si_paged_attn", pool._spec, q.data_ptr(), code, B, H, qs[0], qs[1],
                     page_table.data_ptr(), ts[0], width, lengths.data_ptr(), window, float(sm_scale),
                     out.data_ptr(), _native.ptr(lse), _native.ptr(ws), ws_bytes)

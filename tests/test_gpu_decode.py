@@ -409,7 +409,7 @@ def check_attention(q, pool, table, lengths, window=None, sm_scale=None):
     """Against the oracle, twice: with the table as it is, and with columns of missing pages behind it
     that let the call expect long sequences (whose tiles are dealt to workgroups and joined)."""
     P = pool.page_size
-    more = torch.full((table.shape[0], -(-2200 // P)), -1, dtype=torch.int32, device=table.device)
+    more = torch.full((table.shape[0], -(-3200 // P)), -1, dtype=torch.int32, device=table.device)
     scale = 1 / math.sqrt(pool.head_dim) if sm_scale is None else sm_scale
     want, wlse, weight, reach, peak = R.attend(q, R.pool_values(pool, "k"), R.pool_values(pool, "v"), table, lengths,
                                                scale, window)
@@ -505,7 +505,19 @@ def test_attention_long_and_uneven(lens, dtype):
     check_attention(randn(g, len(lens), 4, 64, dtype=dtype), pool, table, lengths)
 
 
-@pytest.mark.parametrize("longest", [900, 2600])
+@pytest.mark.parametrize("precision,dtype", [("fp32", BF16), ("fp32", F16), ("fp32", F32), ("int8", BF16), ("int4", BF16),
+                                             ("int4", F16)])
+@pytest.mark.parametrize("D,P", [(64, 8), (128, 24), (80, 16), (128, 10)])
+def test_attention_many_items(precision, dtype, D, P):
+    """More items than the chip has CUs."""
+    g = gen(24)
+    lens = torch.randint(0, 100, (90,), generator=torch.Generator().manual_seed(7)).tolist()
+    lens[5] = 300
+    pool, table, lengths = make_cache(g, lens, 3, D, P, precision, dtype)
+    check_attention(randn(g, 90, 6, D, dtype=dtype), pool, table, lengths)
+
+
+@pytest.mark.parametrize("longest", [900, 3300])
 def test_attention_many_sequences(longest):
     """More sequences than a block has threads."""
     g = gen(11)
