@@ -29,6 +29,10 @@ constexpr int kMostParts = 4 * kCUs;  // workgroups of a dealt launch at most
 constexpr double kLog2e = 1.4426950408889634;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// Weights of fp32's range are 2^-24 at most, so that the sum over 2^24 positions of the
+// largest values does not overflow.
+constexpr float kSpare = 24.0f;
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct AttnArgs {
@@ -42,7 +46,7 @@ struct AttnArgs {
   int B, Hk, group, rb;     // rb: row blocks of a group
   int P, window, D, g;
   si_divisor by_page;       // divides by P
-  int64_t pages;
+  int pages;
   float scale, scale_lo;    // times log2(e), and what fp32 leaves of that
   const void* pool[4];      // k, v, scale_k, scale_v
   int sdt;
@@ -147,8 +151,9 @@ __device__ __forceinline__ float max_over_kq(float v) {
 //    [2^14, 2^15): bf16's 8 bits are then exact in fp16 over 2^32. fp16 queries over
 //    bf16 rows are two bf16 parts (NQ = 2), again exact;
 //  * weights w = exp(s - m) sv are two 16-bit parts, hi and what hi leaves. Their
-//    reference m is the maximum of s + log2(sv), so w is at most 2^14 whatever the
-//    rows' scales are, and the parts hold it to 2^-22 (fp16) or 2^-16 (bf16).
+//    reference m is the maximum of s + log2(sv), so the largest is 2^14 in fp16 whatever
+//    the rows' scales are (2^-24 in bf16), and the parts hold a weight to 2^-22 (fp16,
+//    down to 2^-38 of the largest) or 2^-16 (bf16).
 // The k order within a chunk of eight is free as long as both operands have the
 // same: int4's nibbles come out as 1 5 0 4 3 7 2 6.
 //
@@ -220,7 +225,7 @@ struct Engine {
   static constexpr bool kBf = !FP32 && KIND == kBF16;
   static constexpr bool kScaled = KIND == kI8 || KIND == kI4;
   static constexpr int kG = FP32 ? 16 : 8;  // int4 groups of a row at most
-  static constexpr float kRoom = FP32 ? 0.0f : 14.0f;
+  static constexpr float kRoom = FP32 || kBf ? -kSpare : 14.0f;  // weights are up to 2^kRoom
   // bits of a value; words of K per lane and 16 positions, of V per lane and position
   static constexpr int kBits = KIND == kI4 ? 4 : KIND == kI8 ? 8 : KIND == kF32 ? 32 : 16;
   static constexpr int kKW = DP / 4 * kBits / 32, kVW = J * kBits / 32;  // 0: half a word
@@ -240,9 +245,9 @@ struct Engine {
   int32_t row;    // of position lane % 32 (-1: takes no part)
   uint32_t live;  // bit 4 s + i: position s * 16 + 4 kq + i takes part
   int32_t t0, end;  // the wave's position, and where its tiles end
-  // The next tile's table entries: of position lane % 32, or of the four eights. Then
-  // the first rows of the eights that are being loaded.
-  int32_t page[EIGHTS ? 4 : 1], run[EIGHTS ? 4 : 1];
+  // The next tile's table entries and the offsets in their pages: of position lane % 32,
+  // or of the four eights. Then the first rows of the eights that are being loaded.
+  int32_t page[EIGHTS ? 4 : 1], offset[EIGHTS ? 4 : 1], run[EIGHTS ? 4 : 1];
 
   Running<J> st;
   u4 q[NQ][M];
@@ -310,11 +315,15 @@ struct Engine {
   __device__ __forceinline__ void find_pages(const AttnArgs& a, int b, int32_t t, int32_t hi) {
     if constexpr (EIGHTS) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        page[g] = t + 8 * g < hi ? scalar(a.table)[b * a.ts + si_divide(t + 8 * g, a.by_page)] : -1;
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t u = t + 8 * g, p = si_divide(u, a.by_page);
+        page[g] = (int32_t)u < hi ? scalar(a.table)[b * a.ts + p] : -1;
+        offset[g] = (int32_t)(u - p * (uint32_t)a.P);
+      }
     } else {
-      t += threadIdx.x & 31;
-      page[0] = t < hi ? a.table[b * a.ts + si_divide(t, a.by_page)] : -1;
+      const uint32_t u = t + (threadIdx.x & 31), p = si_divide(u, a.by_page);
+      page[0] = (int32_t)u < hi ? a.table[b * a.ts + p] : -1;
+      offset[0] = (int32_t)(u - p * (uint32_t)a.P);
     }
   }
 
@@ -326,8 +335,7 @@ struct Engine {
       bool all = t0 >= lo && t0 + kWaveTokens <= hi;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int32_t u = t0 + 8 * g;
-        run[g] = si_page_row(page[g], a.pages, hk, a.Hk, u - (int32_t)si_divide(u, a.by_page) * a.P, a.P);
+        run[g] = si_page_row(page[g], a.pages, hk, a.Hk, offset[g], a.P);
         all = all && run[g] >= 0;
       }
       if constexpr (kScaled) {
@@ -353,7 +361,7 @@ struct Engine {
       }
     } else {
       row = t >= lo && t < hi
-                ? si_page_row(page[0], a.pages, hk, a.Hk, t - (int32_t)si_divide(t, a.by_page) * a.P, a.P) : -1;
+                ? si_page_row(page[0], a.pages, hk, a.Hk, offset[0], a.P) : -1;
       if (lane < 32) lds_rows[lane] = row;
       wave_sync();
       next_live = 0;
@@ -501,9 +509,8 @@ struct Engine {
       float s[kG], top = 0.0f;
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        if constexpr (!FP32 && NS == 1) s[g] = __uint_as_float(g & 1 ? sc[g / 2] & 0xffff0000u : sc[g / 2] << 16);
-        else s[g] = __uint_as_float(sc[g]);
-        if (row < 0) s[g] = 0.0f;
+        const uint32_t word = row < 0 ? 0u : sc[!FP32 && NS == 1 ? g / 2 : g];
+        s[g] = __uint_as_float(FP32 || NS == 2 ? word : g & 1 ? word & 0xffff0000u : word << 16);
         top = fmaxf(top, s[g]);
       }
       if constexpr (FP32) {
@@ -636,8 +643,13 @@ struct Engine {
       for (int i = 0; i < 4; ++i) {
         float x = acc[s][i];
         if constexpr (FP32) {
-          if constexpr (KIND == kI8) x *= kf[i];
-          x = __builtin_fmaf(x, a.scale, x * a.scale_lo);
+          // the factor in two parts, so that the score is rounded once
+          float f = a.scale, f_lo = a.scale_lo;
+          if constexpr (KIND == kI8) {
+            f = a.scale * kf[i];
+            f_lo = __builtin_fmaf(a.scale, kf[i], -f) + a.scale_lo * kf[i];
+          }
+          x = __builtin_fmaf(x, f, x * f_lo);
         } else {
           x *= qscale;
           if constexpr (kScaled) x *= kf[i];
@@ -827,6 +839,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? E::kBlocks : 1) void paged_attn(At
   int32_t ta = 0, lo, hi;
   if (DEALT) {
     int64_t tiles = 0;
+    if (tid == 0) lds_scan[4] = -1;
     const int chunk = (a.B + 255) / 256;
     const int b0 = tid * chunk, b1 = b0 + chunk < a.B ? b0 + chunk : a.B;
     for (int i = b0; i < b1; ++i) tiles += (int64_t)span_tiles(a, i, &lo, &hi) * per;
@@ -853,6 +866,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? E::kBlocks : 1) void paged_attn(At
     b = (int)uniform(lds_scan[4]);
     item = (int)uniform(lds_scan[5]);
     ta = (int32_t)uniform(lds_scan[6]);
+    if (b < 0) return;  // only if the lengths change while the kernel runs
   } else {
     b = blockIdx.x / per;
     item = blockIdx.x - b * per;
@@ -934,7 +948,9 @@ __global__ __launch_bounds__(64 * W, W == 4 ? E::kBlocks : 1) void paged_attn(At
     ta = 0;
     if (++item == per) {
       item = 0;
-      do { ++b; } while (span_tiles(a, b, &lo, &hi) == 0);  // f < end: one with tiles follows
+      do {  // f < end: a sequence with tiles follows (unless the lengths change meanwhile)
+        if (++b >= a.B) return;
+      } while (span_tiles(a, b, &lo, &hi) == 0);
     }
   }
 }
@@ -1069,8 +1085,8 @@ __global__ __launch_bounds__(256) void paged_attn_any(AttnArgs a, int kind) {
     if ((tid & 63) == 0) red[tid >> 6] = m;
     __syncthreads();
     const float up = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), top);
-    const float ref = up == -INFINITY ? 0.0f : up;
-    const float keep = __builtin_amdgcn_exp2f(top - ref);
+    const float ref = up == -INFINITY ? 0.0f : up + kSpare;
+    const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - up);
     top = up;
     const float w = __builtin_amdgcn_exp2f(s - ref);
     p[tid] = w;
@@ -1095,7 +1111,7 @@ __global__ __launch_bounds__(256) void paged_attn_any(AttnArgs a, int kind) {
     const int d = tid + e * 256;
     if (d < a.D) store_any(a.out, a.qdt, out * a.D + d, sum == 0.0f ? 0.0f : o[e] / sum);
   }
-  if (tid == 0 && a.lse) a.lse[out] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  if (tid == 0 && a.lse) a.lse[out] = sum == 0.0f ? -INFINITY : (top + kSpare + log2f(sum)) * kLn2;
 }
 
 // Whether items' tiles are dealt (and joined), by the most tiles one can have: whole
@@ -1107,7 +1123,7 @@ __global__ __launch_bounds__(256) void paged_attn_any(AttnArgs a, int kind) {
 bool dealt(int64_t items, int64_t capacity, int64_t window) {
   const int64_t most = window > 0 && window < capacity ? window : capacity;
   const int64_t limit = 6 + items / 16;
-  return most > (limit < 24 ? limit : 24) * kTile;
+  return most > (limit < 20 ? limit : 20) * kTile;
 }
 
 template <class E>
@@ -1118,8 +1134,8 @@ int launch(AttnArgs a, bool deal, hipStream_t st) {
     paged_attn<E, true, 4><<<a.most, 256, 0, st>>>(a);
     const int rows = a.group < kRows ? a.group : kRows;
     paged_join<<<dim3((unsigned)items, (unsigned)rows), 256, 0, st>>>(a);
-  } else if (items <= kCUs) {
-    // eight waves where a CU has one item at most: 1000 positions of 24 x 8 items 16.9
+  } else if (items <= kCUs && a.capacity > kTile && (a.window == 0 || a.window > kTile)) {
+    // eight waves where there is work for them and a CU has one item at most: 1000 positions of 24 x 8 items 16.9
     // us for 21.1 with four, of 64 x 8 items 34.2 for 30.1
     paged_attn<E, false, 8><<<(unsigned)items, 512, 0, st>>>(a);
   } else {
@@ -1190,7 +1206,7 @@ extern "C" int si_paged_attn(const si_page_pool* pool, const void* q, int q_dtyp
   a.window = (int)window;
   a.D = (int)p.D;
   a.g = (int)p.group;
-  a.pages = p.pages;
+  a.pages = (int)p.pages;
   a.scale = (float)(scale * kLog2e);
   a.scale_lo = (float)(scale * kLog2e - a.scale);
   a.pool[0] = p.k;

@@ -24,8 +24,8 @@ struct PoolArgs {
   char* vo;
   int64_t ks[2], vs[2];   // elements between tokens and heads
   const int64_t* slots;
-  int64_t T, pages;
-  int H, P, D, g, prec;
+  int64_t T;
+  int pages, H, P, D, g, prec;
   int sdt, odt;           // pool type; output type (read)
   int lpg, nl;            // lanes of an int4 group and of a row
   Buckets pool;           // the pool's tensors in the slots of `prec`
@@ -328,7 +328,7 @@ PoolArgs pool_args(const si_page_pool& p, int64_t T, const int64_t* slots) {
   a.T = T;
   a.H = (int)p.heads;
   a.D = (int)p.D;
-  a.pages = p.pages;
+  a.pages = (int)p.pages;
   a.P = (int)p.page_size;
   a.prec = (int)p.precision;
   a.g = (int)p.group;

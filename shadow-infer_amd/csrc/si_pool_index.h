@@ -14,17 +14,17 @@
 
 // Row of (page, head, offset) in the pool's [pages, heads, page_size] rows, -1 for
 // a page outside the pool. Pools have fewer than 2^31 rows.
-SI_HD int32_t si_page_row(int64_t page, int64_t pages, int32_t head, int32_t heads, int32_t offset,
+SI_HD int32_t si_page_row(int32_t page, int32_t pages, int32_t head, int32_t heads, int32_t offset,
                           int32_t page_size) {
-  if (page < 0 || page >= pages) return -1;
-  return (int32_t)((page * heads + head) * page_size + offset);
+  if ((uint32_t)page >= (uint32_t)pages) return -1;
+  return (page * heads + head) * page_size + offset;
 }
 
 // Row of a slot (page * page_size + offset) of one head, -1 for a slot outside.
-SI_HD int32_t si_slot_row(int64_t slot, int64_t pages, int32_t head, int32_t heads, int32_t page_size) {
-  if (slot < 0 || slot >= pages * page_size) return -1;
+SI_HD int32_t si_slot_row(int64_t slot, int32_t pages, int32_t head, int32_t heads, int32_t page_size) {
+  if (slot < 0 || slot >= (int64_t)pages * page_size) return -1;
   const uint32_t s = (uint32_t)slot, p = s / (uint32_t)page_size;
-  return si_page_row(p, pages, head, heads, (int32_t)(s - p * (uint32_t)page_size), page_size);
+  return si_page_row((int32_t)p, pages, head, heads, (int32_t)(s - p * (uint32_t)page_size), page_size);
 }
 
 // Positions [lo, hi) that take part: the last `window` (0: all) of `length`, which

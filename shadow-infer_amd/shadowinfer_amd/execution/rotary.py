@@ -117,11 +117,23 @@ class RotaryEmbedding:
         self.angles = tuple(angles)  # radians per position of each pair
         self.device = torch.device(device)
         # turns per position, in fp64 on the device
-        self.turns = torch.tensor([x / (2.0 * math.pi) for x in angles], dtype=torch.float64,
+        self._turns = torch.tensor([x / (2.0 * math.pi) for x in angles], dtype=torch.float64,
                                   device=self.device)
+        self._bind()
+
+    def _bind(self) -> None:
         self._spec = ctypes.create_string_buffer(struct.pack(  # si_rotation
-            "=qqQd", size // 2, 1 if layout == "interleaved" else 0, self.turns.data_ptr(),
-            self.value_factor))
+            "=qqQd", self.rotary_dim // 2, 1 if self.layout == "interleaved" else 0,
+            self._turns.data_ptr(), self.value_factor))
+
+    def __getstate__(self) -> dict:
+        return {k: v for k, v in self.__dict__.items() if k != "_spec"}
+
+    def __setstate__(self, state: dict) -> None:  # a copy has a tensor of its own
+        self.__dict__.update(state)
+        self._bind()
+
+    turns = property(lambda self: self._turns)
 
     def _rows(self, x: torch.Tensor, shape, what: str, inplace: bool):
         """(source, output, their si_rotary_rows). The source may be a copy."""
@@ -170,7 +182,7 @@ class RotaryEmbedding:
         every row of a batch, ``[S]``; any value. ``transpose=True`` turns the
         other way: the gradient of this call with respect to its input, and,
         where ``value_factor`` is 1, its inverse. ``inplace=True`` writes into q
-        and k. Not recorded by autograd."""
+        and k, which share no values then. Not recorded by autograd."""
         index = q.get_device()
         if index < 0:
             _native.require_device(q, "RotaryEmbedding")
@@ -189,6 +201,8 @@ class RotaryEmbedding:
             if len(kshape) != len(shape) or kshape[:-2] != lead or kshape[-1] != self.head_dim:
                 raise ValueError("q and k must hold the same tokens, got "
                                  f"{tuple(shape)} and {tuple(kshape)}")
+            if inplace and k.data_ptr() == q.data_ptr() and k.numel():
+                raise ValueError("q and k cannot be the same values in place")
         wide, pb, ps = self.check_positions(positions, lead, index)
         # sources stay bound until the launch is queued
         src_q, out_q, rows_q = self._rows(q, shape, "q", inplace)

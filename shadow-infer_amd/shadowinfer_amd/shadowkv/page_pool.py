@@ -64,10 +64,20 @@ class KVPagePool:
         self._k, self._v = zeros(row, payload), zeros(row, payload)
         self._sk = None if scales is None else zeros(scales, dtype)
         self._sv = None if scales is None else zeros(scales, dtype)
+        self._bind()
+
+    def _bind(self) -> None:
         self._spec = _SPEC(self.num_pages, self.num_heads, self.page_size, self.head_dim,
-                           _PREC_CODE[precision], self._dtype_code, self.int4_group_size,
+                           _PREC_CODE[self.precision], self._dtype_code, self.int4_group_size,
                            *(_native.ptr(t) or 0 for t in (self._k, self._v, self._sk, self._sv)))
         self._index = self._k.get_device()
+
+    def __getstate__(self) -> dict:
+        return {k: v for k, v in self.__dict__.items() if k not in ("_spec", "_index")}
+
+    def __setstate__(self, state: dict) -> None:  # a copy has tensors of its own
+        self.__dict__.update(state)
+        self._bind()
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
@@ -102,7 +112,7 @@ class KVPagePool:
         twice in one call: which of its rows stays, and with which scale, would
         be open. With ``rotary`` (a RotaryEmbedding) K is rotated to
         ``positions`` ``[T]`` on its way, to the bytes that rotating first would
-        give."""
+        give. Not recorded by autograd."""
         index = self._index
         if k.get_device() < 0 or index < 0:
             _native.require_device(k, "KVPagePool.write")

@@ -30,7 +30,8 @@ def paged_attention(q: torch.Tensor, pool: KVPagePool, page_table: torch.Tensor,
     ``window``: only the last so many positions. Positions of a page outside the
     pool (-1: dropped) take no part, lengths are cut to the table, negative ones
     are 0. A sequence without positions gives zeros and -inf. Several query heads
-    of one kv head share its read; scores, softmax and sums are fp32."""
+    of one kv head share its read; scores, softmax and sums are fp32. Not recorded by
+    autograd."""
     index = q.get_device()
     if index < 0:
         _native.require_device(q, "paged_attention")

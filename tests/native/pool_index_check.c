@@ -29,9 +29,9 @@ static uint64_t rnd(uint64_t n) {
 }
 
 static void rows(void) {
-  const int64_t pages = 1 + rnd(9);
+  const int32_t pages = 1 + (int32_t)rnd(9);
   const int heads = 1 + (int)rnd(5), P = 1 + (int)rnd(20);
-  const int64_t n = pages * heads * P;
+  const int64_t n = (int64_t)pages * heads * P;
   char* seen = calloc((size_t)n, 1);
   for (int h = 0; h < heads; ++h)
     for (int64_t s = -3; s < pages * P + 3; ++s) {
@@ -39,10 +39,11 @@ static void rows(void) {
       if (s < 0 || s >= pages * P) { CHECK(r == -1); continue; }
       CHECK(r >= 0 && r < n && !seen[r]);
       seen[r] = 1;
-      CHECK(r == si_page_row(s / P, pages, h, heads, (int32_t)(s % P), P));
+      CHECK(r == si_page_row((int32_t)(s / P), pages, h, heads, (int32_t)(s % P), P));
     }
   free(seen);
-  for (int64_t p = -2; p < pages + 2; ++p)
+  CHECK(si_page_row(-2147483647 - 1, pages, 0, heads, 0, P) < 0 && si_page_row(2147483647, pages, 0, heads, 0, P) < 0);
+  for (int32_t p = -2; p < pages + 2; ++p)
     CHECK((si_page_row(p, pages, 0, heads, 0, P) >= 0) == (p >= 0 && p < pages));
 }
 

@@ -12,7 +12,9 @@ chains of n positions; weights may be carried as two 16-bit parts where the quer
 have 16 bits (2^-16). The bound is that factor times sum p |v|, plus the result's half step.
 """
 
+import copy
 import math
+import pickle
 
 import numpy as np
 import pytest
@@ -192,6 +194,28 @@ def test_rotary_refusals():
         rope(p, torch.zeros(4, 64, 2, device="cuda").transpose(1, 2), inplace=True)
     with pytest.raises(ValueError):
         RotaryEmbedding(64, device="cpu")(p, x)
+    with pytest.raises(ValueError):
+        rope(p, x, x, inplace=True)
+
+
+def test_copies_have_tensors_of_their_own():
+    """copy.deepcopy and pickle rebuild what the calls hand to the library."""
+    g = gen(9)
+    x = randn(g, 5, 2, 64, dtype=BF16)
+    p = torch.arange(5, device="cuda")
+    rope, pool = RotaryEmbedding(64), KVPagePool(2, 2, 64, page_size=4)
+    pool.write(x, x, p)
+    want = rope(p, x), pool.read(p)
+    for make in (copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))):
+        r, q = make(rope), make(pool)
+        assert r.turns.data_ptr() != rope.turns.data_ptr() and q.k.data_ptr() != pool.k.data_ptr()
+        assert torch.equal(r(p, x), want[0]) and torch.equal(q.read(p)[0], want[1][0])
+        q.write(-x, x, p)
+        assert torch.equal(pool.read(p)[0], want[1][0]) and not torch.equal(q.read(p)[0], want[1][0])
+        with pytest.raises(AttributeError):
+            r.turns = None
+        with pytest.raises(AttributeError):
+            q.k = None
 
 
 # --------------------------------------------------------------------- pool
@@ -576,6 +600,23 @@ def test_attention_scales(qt, dtype, precision, qs, ks, vs):
     v *= torch.logspace(-2, 0, pool.num_slots, device="cuda")[:, None, None].to(dtype)
     pool.write(k, v, slots)
     check_attention(randn(g, 2, 8, D, dtype=qt, scale=qs), pool, table, lengths)
+
+
+@pytest.mark.parametrize("dtype,precision,size", [(BF16, "fp32", 2.0 ** 126), (F32, "fp32", 2.0 ** 126),
+                                                  (BF16, "int8", 2.0 ** 126), (F16, "fp32", 32768.0),
+                                                  (BF16, "int4", 2.0 ** 126), (BF16, "fp32", 2.0 ** -100),
+                                                  (BF16, "int8", 2.0 ** -70), (BF16, "int4", 2.0 ** -70)])
+@pytest.mark.parametrize("D", [64, 45])
+def test_attention_values_at_the_range_ends(dtype, precision, size, D):
+    """Values near the type's largest and down to 2^-100 come out finite and as exact as others."""
+    g = gen(25)
+    pool, table, lengths = make_cache(g, [70, 300], 1, D, 16, precision, dtype)
+    slots = torch.arange(pool.num_slots, device="cuda")
+    k = randn(g, pool.num_slots, 1, D, dtype=dtype)
+    v = (torch.rand(pool.num_slots, 1, D, generator=g, device="cuda") * 2 - 1) * size
+    pool.write(k, v.to(dtype), slots)
+    out = check_attention(randn(g, 2, 4, D, dtype=dtype), pool, table, lengths)
+    assert torch.isfinite(out).all() and (out != 0).any()
 
 
 @pytest.mark.parametrize("precision", ["fp32", "int8"])
