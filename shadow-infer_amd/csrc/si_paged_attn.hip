@@ -232,18 +232,18 @@ struct Engine {
   static constexpr int kVW1 = kVW ? kVW : 1;
   static constexpr int kUnit = 8 * kBits / 32;  // words of eight values
 
-  // A wave's LDS: rows [32], then per position K's factor and V's factor, and int4's
+  // A wave's LDS: rows [32], then per position K's factor, V's and its logarithm, and int4's
   // scales as [32][kG] for K and [kG][32] for V, s' in NS fp16 parts each or
   // fp32.
   static constexpr int kLdsScale = 32 * 4;
-  static constexpr int kLdsParts = kLdsScale + (kScaled ? 2 * 32 * 4 : 0);
+  static constexpr int kLdsParts = kLdsScale + (kScaled ? 3 * 32 * 4 : 0);
   static constexpr int kLds = kLdsParts + (KIND == kI4 ? 2 * 32 * kG * (FP32 ? 4 : 2 * NS) : 0);
 
   uint32_t k[2][kKW], v[2][4][kVW1];  // a tile's rows
   uint32_t sc[KIND == kI4 ? (FP32 ? 16 : NS == 1 ? 4 : 8) : 1];
-  uint32_t next_live;
   int32_t row;    // of position lane % 32 (-1: takes no part)
-  uint32_t live;  // bit 4 s + i: position s * 16 + 4 kq + i takes part
+  uint32_t live, next_live;  // bit 4 s + i: position s * 16 + 4 kq + i takes part
+  bool full, next_full;      // all positions of the tile do
   int32_t t0, end;  // the wave's position, and where its tiles end
   // The next tile's table entries and the offsets in their pages: of position lane % 32,
   // or of the four eights. Then the first rows of the eights that are being loaded.
@@ -346,6 +346,7 @@ struct Engine {
         const int32_t lower = lane & 8 ? r[1] : r[0], upper = lane & 8 ? r[3] : r[2], first = lane & 16 ? upper : lower;
         row = first >= 0 && t >= lo && t < hi ? first + (lane & 7) : -1;
       }
+      next_full = all;
       next_live = 0xffu;
       if (!all) {
         next_live = 0;
@@ -373,6 +374,7 @@ struct Engine {
         for (int i = 0; i < 4; ++i)
           if (r[i] >= 0) next_live |= 1u << (4 * s + i);
       }
+      next_full = __all(next_live == 0xffu);
     }
   }
 
@@ -456,6 +458,7 @@ struct Engine {
     const char* vp = reinterpret_cast<const char*>(a.pool[1]);
     const int64_t n = row_bytes(a);
     live = next_live;
+    full = next_full;
     const bool in = EXACT || c * J < a.D;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -483,23 +486,16 @@ struct Engine {
   }
 
   // The factors of the lane's own positions s * 16 + 4 kq + i (j: 0 K, 1 V): an int8 row's
-  // scale, 2^e of an int4 row's, 0 for a position that takes no part.
+  // scale, 2^e of an int4 row's, 0 for a position that takes no part. j 2: log2 of V's.
   __device__ __forceinline__ static f32x4 factors(const char* lds, int j, int s) {
     const int kq = (threadIdx.x & 63) >> 4;
     return *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + kLdsScale) + 32 * j + s * 16 + kq * 4);
   }
 
-  // At least log2 of a factor: 1 + the mantissa is at most 0.0861 below 2^mantissa. (A
-  // factor below 2^-80 or not a number: its weight needs no more room than this.)
-  __device__ __forceinline__ static float log2_bound(float f) {
-    const float x = fmaxf(__builtin_fmaf((float)(int)__float_as_uint(f), 0x1p-23f, -126.913f), -80.0f);
-    return f < INFINITY ? x : -80.0f;
-  }
-
   // The tile's scales into the wave's LDS.
   __device__ __forceinline__ void place_scales(const AttnArgs& a, char* lds) const {
     const int lane = threadIdx.x & 63, t = lane & 31;
-    float* factor = reinterpret_cast<float*>(lds + kLdsScale);  // [2][32]
+    float* factor = reinterpret_cast<float*>(lds + kLdsScale);  // [3][32]
     float f = 1.0f;
     if constexpr (KIND == kI8) {
       f = a.sdt == SI_DT_F32 ? __uint_as_float(sc[0])
@@ -537,6 +533,8 @@ struct Engine {
       }
     }
     factor[lane] = f;
+    // (a factor below 2^-80 or not a number: its weight needs no more room than this)
+    if (!FP32 && lane >= 32) factor[32 + lane] = f < INFINITY ? fmaxf(__builtin_amdgcn_logf(f), -80.0f) : -80.0f;
     wave_sync();
   }
 
@@ -629,15 +627,16 @@ struct Engine {
 
   // Its weights and their products with the values.
   __device__ __forceinline__ void values(const AttnArgs& a, const char* lds, const f32x4* acc) {
-    float w[8], y[8], top = st.m;
+    float w[8], y[8], bound[8], top = st.m;
     f32x4 vf[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      f32x4 kf = {1.0f, 1.0f, 1.0f, 1.0f};
+      f32x4 kf = {1.0f, 1.0f, 1.0f, 1.0f}, lg = {0.0f, 0.0f, 0.0f, 0.0f};
       vf[s] = kf;
       if constexpr (kScaled) {
         kf = factors(lds, 0, s);
         vf[s] = factors(lds, 1, s);
+        if constexpr (!FP32) lg = factors(lds, 2, s);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -654,11 +653,17 @@ struct Engine {
           x *= qscale;
           if constexpr (kScaled) x *= kf[i];
         }
-        if (!(live >> (4 * s + i) & 1)) x = -INFINITY;
         y[4 * s + i] = x;
-        top = fmaxf(top, kScaled && !FP32 ? x + log2_bound(vf[s][i]) : x);
+        bound[4 * s + i] = lg[i];
       }
     }
+    if (!full) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(live >> i & 1)) y[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, y[i] + bound[i]);
     top = max_over_kq(top);
     if (__any(top > st.m)) {
       const float keep = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m - top);
@@ -697,7 +702,7 @@ struct Engine {
         float x[J];
         widen<KIND, J>(v[s][i], x);
         // rows that take no part count as zeros, whatever they hold
-        const bool dead = !kScaled && !(live >> (4 * s + i) & 1);
+        const bool dead = !kScaled && !full && !(live >> (4 * s + i) & 1);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           if constexpr (KIND == kI4) x[j] *= vs[s][i];
@@ -742,7 +747,7 @@ struct Engine {
         v_pairs(v[t >> 1][2 * (t & 1)], v[t >> 1][2 * (t & 1) + 1], i, vv[t]);
         if constexpr (!kScaled) {
           // rows that take no part count as zeros, whatever they hold
-          if (live != 0xffu) {
+          if (!full) {
             const uint32_t mask = (live >> (2 * t) & 1 ? 0xffffu : 0u) | (live >> (2 * t + 1) & 1 ? 0xffff0000u : 0u);
 #pragma unroll
             for (int j = 0; j < kJG; ++j) vv[t][j] &= mask;
