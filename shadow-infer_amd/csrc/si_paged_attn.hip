@@ -18,9 +18,9 @@
 //
 // Measured, 32 query heads of 128, bf16: 131072 positions of 8 kv heads, int8 58 us (4.7
 // TB/s of cache, 7.7 us more for the join), int4 54, bf16 106 (5.1 TB/s); 16 sequences of
-// 8192 over 32 kv heads, int8 201 (5.15 TB/s); 64 uneven sequences up to 4096, int4 73: a
-// tile costs a wave about 640 VALU instructions, and the VALU is busy 64% of that kernel
-// and 85% of a wave's life. 100 positions: 6.5.
+// 8192 over 32 kv heads, int8 201 (5.15 TB/s); 64 uneven sequences up to 4096, int4 73: 32
+// positions cost a wave about 580 VALU instructions, which keep a SIMD busy 80% of the
+// time that its waves live. 100 positions: 6.5.
 #include "si_pool_args.h"
 #include "si_pool_index.h"
 #include "si_kv_common.h"
@@ -227,9 +227,10 @@ template <int KIND, int DP_, bool EXACT, bool EIGHTS, bool FP32, int NQ, int NS>
 struct Engine {
   static constexpr int kKind = KIND;
   static constexpr int DP = DP_, J = DP / 16, M = DP / 32;
-  // Blocks of a CU, for the registers' bound and the dealing. Two against three: int4
-  // rows 95 / 82 us (64 uneven sequences), int8 76 / 68 (131072 positions), bf16 104 / 122.
-  // fp32 rows with one 89, with two (and spills) 152.
+  // Blocks of a CU, for the registers' bound and the dealing. Two against three, us:
+  // int4 88 / 77 (64 uneven sequences) and 58.7 / 54 (131072 positions); int8 64.4 / 65.8
+  // and 197.5 / 203.8 (16 x 8192) at 128 wide, but 28.1 / 27.3 at 64, 54.8 / 50.6 at 80 and
+  // 97.4 / 92.1 with fp32 queries; bf16 106.4 / 108.7. fp32 rows, one against two: 90 / 125.
   static constexpr int kBlocks = KIND == kF32 ? 1 : KIND == kI8 || (KIND == kI4 && !FP32) ? 3 : 2;
   static constexpr bool kBf = !FP32 && KIND == kBF16;
   static constexpr bool kScaled = KIND == kI8 || KIND == kI4;

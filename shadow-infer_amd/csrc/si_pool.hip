@@ -8,7 +8,7 @@
 // slot outside the pool is skipped when written and gives zeros when read.
 //
 // Both kernels move every byte once and are bound by HBM, at few tokens by the
-// launch and one chain of loads (64 tokens x 8 heads: 3.8 us each).
+// launch and one chain of loads (64 tokens x 8 heads: 3.8 and 3.9 us).
 #include "si_pool_args.h"
 #include "si_pool_index.h"
 #include "si_rotate.h"
@@ -137,7 +137,7 @@ __device__ __forceinline__ void write_row(const PoolArgs& a, int lane, int32_t r
 // blocks), so rows that share a cache line of the pool are written together. The rows
 // are loaded beside their slots, non-temporal: written and read back, 8192 x 32 rows of
 // 128 bf16 take 76 us as int4 (78 with plain loads), 74 as int8 (81) and 94 unquantized
-// (109), 4.6 to 5.7 TB/s; two rows a thread instead of one cost 2%.
+// (109), 4.6 to 5.7 TB/s; two rows a thread took 75.7, 75 and 96.
 template <int DT, int LPR>
 __global__ __launch_bounds__(256) void pool_write(PoolArgs a) {
   constexpr int RPP = 256 / LPR;
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void pool_write(PoolArgs a) {
 }
 
 // With a rotation: block = `tb` tokens and all their heads, whose cosines it
-// computes once (2048 tokens x 8 heads of 128 bf16: 7.4 us for 16.8 MB, 3 of them launch).
+// computes once (2048 tokens x 8 heads of 128 bf16: 7.4 us for 16.8 MB).
 template <int DT, int LPR>
 __global__ __launch_bounds__(256) void pool_write_rotated(PoolArgs a, int tb) {
   constexpr int RPP = 256 / LPR;

@@ -7,9 +7,10 @@
 // tokens x 40 heads of 128 bf16: 41 us, 4.1 TB/s) and the launch short ones (one token:
 // 3.6 us). The angles come from the positions, not from a table: a block computes the
 // cosines of its tokens once, in 64 bits, keeps them in LDS and uses them for every
-// head. Stores are plain, as what follows reads the rows: non-temporal ones take the
-// kernel to 38 us but a reader behind it from 25 to 32; write-through ones 94. Four
-// rows a thread took 53 us, one 41.3.
+// head. Stores are plain, as what follows reads the rows: with non-temporal ones
+// the kernel alone took 36 to 38 us, but together with a reader behind it 70.8 against
+// 66.4; with device-scope ones 94. Four rows a thread took 53 us; one took 41 (interleaved)
+// and 38.2 against 40.1 (half), but 4.66 against 4.58 at 1003 tokens x 24 heads of 80.
 #include "si_rotate.h"
 
 namespace si {
